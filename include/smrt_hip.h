@@ -265,6 +265,74 @@ int  smrt_smote_rows_f64(const double* X_dev, int64_t n_x, int64_t ldx, int64_t 
                          const int64_t* nbr_idx_dev, const double* r_dev, int64_t n_rows, int32_t mode,
                          double* out_dev, int64_t ldo, void* hip_stream);
 
+/* ---- layer operators (no counterpart in the reference, whose layers exist only inside its TensorFlow graph: layer.py:348-368).
+ * The dense layer, layer norm and the 8-bit form of activations, each with its gradients, on matrices of the caller's: what
+ * the handles above run inside one net, for nets that are put together from layers.
+ *
+ * Types: SMRT_F32, SMRT_BF16, SMRT_F16; sums are fp32.  Matrices are row-major DEVICE memory, elements of a row next to each
+ * other, a leading dimension (in elements) for each; rows may start at any element.  Work is queued on hip_stream, nothing is
+ * allocated, nothing waits: the calls can be captured into a graph.  Workspaces are the caller's, not shared by calls that may
+ * run at the same time.  Sizes may be 0.  Returns 0, or -1 (bad argument, nothing was done) or -2 (launch failed).
+ *
+ * Groups: with `ends` (device, int64[groups]) group g is the rows [ends[g-1], ends[g]) (from row 0 for g = 0) and has its own
+ * weight, w + g * w_stride, and bias, bias + g * bias_stride.  The kernels clamp an end to [the one before, rows], so no
+ * content of `ends` makes them leave the matrices.  Rows behind the last end are in no group: y, a and dx are zero there, or
+ * with keep_rest != 0 y and dx are left as they were.
+ *
+ * The 8-bit form of a matrix [rows][n]: q int8 [rows][ldq], ldq >= n rounded up to 32 (the pad is zero), and one scale byte per 32
+ * columns, scale [rows][ld_scale].  A value is q * 2^(byte - 127), q in [-127, 127], with the smallest power that holds the 32
+ * columns' largest magnitude (not below 2^-126; 2^-24 in SMRT_F16); halves round to even.  Byte 255: the block held an infinity
+ * or a NaN, and all of it stands for NaN. */
+enum { SMRT_F32 = 0, SMRT_BF16 = 1, SMRT_F16 = 2 };
+
+typedef struct smrt_dense {
+    int32_t dtype, activation;                      /* SMRT_F32.., SMRT_ACT_* */
+    int64_t rows, k, n;                             /* x [rows][k], W [k][n], y [rows][n] */
+    int32_t groups, keep_rest;                      /* groups in [1, 65535] */
+    const int64_t* ends;                            /* NULL: one group of all rows */
+    const void* x; int64_t ldx;                     /* backward: x_scale != NULL means x is the 8-bit form (int8) */
+    const uint8_t* x_scale; int64_t ld_x_scale;
+    const void* w; int64_t ldw, w_stride;
+    const void* bias; int64_t bias_stride;          /* NULL: none.  bias_stride is also db's */
+    const void* residual; int64_t ldr;              /* forward, NULL: none */
+    void* y; int64_t ldy;                           /* forward */
+    void* a; int64_t lda;                           /* act(x W + b): written by forward (NULL: not), read by backward;
+                                                     * a_scale != NULL means the 8-bit form */
+    uint8_t* a_scale; int64_t ld_a_scale;
+    const void* grad; int64_t ldg;                  /* backward: d loss / d y */
+    void* dx; int64_t lddx;                         /* backward, each NULL: not wanted */
+    void* dw; int64_t lddw, dw_stride;
+    void* db;
+} smrt_dense;
+/* y = act(x W + b) + residual.  y may be the residual itself, and overlaps no other input. */
+int     smrt_dense_forward(const smrt_dense* args, void* hip_stream);
+/* From grad: dz = grad * act'(.) taken at the value of a (not read for SMRT_ACT_IDENTITY), dx = dz W^T, dw = x^T dz, db = column
+ * sums of dz.  The residual's gradient is grad.  A 16-bit dz is rounded once to dtype, as a product's operand. */
+int64_t smrt_dense_backward_workspace(const smrt_dense* args);      /* bytes, or -1 */
+int     smrt_dense_backward(const smrt_dense* args, void* workspace, int64_t workspace_bytes, void* hip_stream);
+
+typedef struct smrt_layer_norm {
+    int32_t dtype, weight_f32;                      /* weight, bias, dw, db: of dtype, or fp32 */
+    int64_t rows, n;                                /* n in [1, 32768] */
+    float   eps;
+    const void* x; int64_t ldx;                     /* backward: x_scale != NULL means x is the 8-bit form (int8) */
+    const uint8_t* x_scale; int64_t ld_x_scale;
+    const void* weight; const void* bias;           /* [n], NULL: 1 and 0 */
+    void* y; int64_t ldy;                           /* forward; may be x itself */
+    float* mean; float* rstd;                       /* [rows]: written by forward, read by backward */
+    const void* grad; int64_t ldg;                  /* backward */
+    void* dx; int64_t lddx; void* dw; void* db;     /* backward, each NULL: not wanted */
+} smrt_layer_norm;
+/* y = (x - mean) * rstd * weight + bias with each row's mean and rstd = 1 / sqrt(variance + eps) */
+int     smrt_layer_norm_forward(const smrt_layer_norm* args, void* hip_stream);
+int64_t smrt_layer_norm_backward_workspace(const smrt_layer_norm* args);
+int     smrt_layer_norm_backward(const smrt_layer_norm* args, void* workspace, int64_t workspace_bytes, void* hip_stream);
+
+int  smrt_pack_rows(int32_t dtype, const void* x, int64_t ldx, int64_t rows, int64_t n, int8_t* q, int64_t ldq, uint8_t* scale,
+                    int64_t ld_scale, void* hip_stream);
+int  smrt_unpack_rows(int32_t dtype, const int8_t* q, int64_t ldq, const uint8_t* scale, int64_t ld_scale, int64_t rows, int64_t n,
+                      void* x, int64_t ldx, void* hip_stream);
+
 /* ---- diagnostics: achievable peaks and the latency floor the roofline figures are quoted against.
  * No counterpart in the reference; nothing on the product path calls them.
  *   smrt_diag_mfma_peak     : register-resident v_mfma_f32_32x32x2_f32 loop on every CU -> TFLOP/s actually reachable.

@@ -29,6 +29,8 @@ EXPORTS = [
     "smrt_vae_set_stream", "smrt_vae_encode", "smrt_vae_decode",
     "smrt_vae_generate", "smrt_vae_generate_noalloc", "smrt_vae_generate_noalloc_max_rows", "smrt_vae_sample_eps", "smrt_vae_last_epoch_launches", "smrt_vae_profile_epochs",
     "smrt_assemble_rows", "smrt_assemble_rows_part", "smrt_assemble_rows_synth_range", "smrt_assemble_rows_f64", "smrt_all_finite", "smrt_rng_normal", "smrt_rng_permutation", "smrt_knn_f64", "smrt_smote_rows_f64", "smrt_diag_mfma_peak", "smrt_diag_mfma_peak_16x16x4", "smrt_diag_hbm_bandwidth", "smrt_diag_step_floor",
+    "smrt_dense_forward", "smrt_dense_backward", "smrt_dense_backward_workspace", "smrt_layer_norm_forward", "smrt_layer_norm_backward",
+    "smrt_layer_norm_backward_workspace", "smrt_pack_rows", "smrt_unpack_rows",
     "smrt_last_error", "smrt_version",
 ]
 
@@ -40,6 +42,31 @@ class VaeCfg(C.Structure):
         ("learning_rate", C.c_float), ("l2_penalty", C.c_float), ("clip", C.c_int32),
         ("gclip_min", C.c_float), ("gclip_max", C.c_float), ("bce_lo", C.c_float), ("bce_hi", C.c_float),
         ("dropout_keep", C.c_float), ("seed", C.c_uint64), ("max_batch", C.c_int32), ("model", C.c_int32),
+    ]
+
+
+class Dense(C.Structure):
+    """``smrt_dense`` of include/smrt_hip.h."""
+    _fields_ = [
+        ("dtype", C.c_int32), ("activation", C.c_int32), ("rows", C.c_int64), ("k", C.c_int64), ("n", C.c_int64),
+        ("groups", C.c_int32), ("keep_rest", C.c_int32), ("ends", C.c_void_p),
+        ("x", C.c_void_p), ("ldx", C.c_int64), ("x_scale", C.c_void_p), ("ld_x_scale", C.c_int64),
+        ("w", C.c_void_p), ("ldw", C.c_int64), ("w_stride", C.c_int64), ("bias", C.c_void_p), ("bias_stride", C.c_int64),
+        ("residual", C.c_void_p), ("ldr", C.c_int64), ("y", C.c_void_p), ("ldy", C.c_int64),
+        ("a", C.c_void_p), ("lda", C.c_int64), ("a_scale", C.c_void_p), ("ld_a_scale", C.c_int64),
+        ("grad", C.c_void_p), ("ldg", C.c_int64), ("dx", C.c_void_p), ("lddx", C.c_int64),
+        ("dw", C.c_void_p), ("lddw", C.c_int64), ("dw_stride", C.c_int64), ("db", C.c_void_p),
+    ]
+
+
+class LayerNorm(C.Structure):
+    """``smrt_layer_norm`` of include/smrt_hip.h."""
+    _fields_ = [
+        ("dtype", C.c_int32), ("weight_f32", C.c_int32), ("rows", C.c_int64), ("n", C.c_int64), ("eps", C.c_float),
+        ("x", C.c_void_p), ("ldx", C.c_int64), ("x_scale", C.c_void_p), ("ld_x_scale", C.c_int64),
+        ("weight", C.c_void_p), ("bias", C.c_void_p), ("y", C.c_void_p), ("ldy", C.c_int64),
+        ("mean", C.c_void_p), ("rstd", C.c_void_p), ("grad", C.c_void_p), ("ldg", C.c_int64),
+        ("dx", C.c_void_p), ("lddx", C.c_int64), ("dw", C.c_void_p), ("db", C.c_void_p),
     ]
 
 
@@ -114,6 +141,14 @@ def load():
     lib.smrt_assemble_rows_synth_range.argtypes = [vp, i64, i64, i64, i64, vp, i64, vp, i32, i64, i64]
     lib.smrt_rng_normal.argtypes = [vp, C.POINTER(i32), C.POINTER(i32), C.POINTER(C.c_double), C.c_double, C.c_double, vp, i64, i32]
     lib.smrt_rng_permutation.argtypes = [vp, C.POINTER(i32), vp, i64]
+    lib.smrt_dense_forward.argtypes = [C.POINTER(Dense), vp]
+    lib.smrt_dense_backward.argtypes = [C.POINTER(Dense), vp, i64, vp]
+    lib.smrt_dense_backward_workspace.argtypes = [C.POINTER(Dense)]; lib.smrt_dense_backward_workspace.restype = i64
+    lib.smrt_layer_norm_forward.argtypes = [C.POINTER(LayerNorm), vp]
+    lib.smrt_layer_norm_backward.argtypes = [C.POINTER(LayerNorm), vp, i64, vp]
+    lib.smrt_layer_norm_backward_workspace.argtypes = [C.POINTER(LayerNorm)]; lib.smrt_layer_norm_backward_workspace.restype = i64
+    lib.smrt_pack_rows.argtypes = [i32, vp, i64, i64, i64, vp, i64, vp, i64, vp]
+    lib.smrt_unpack_rows.argtypes = [i32, vp, i64, vp, i64, i64, i64, vp, i64, vp]
     _lib = lib
     return lib
 

@@ -1,0 +1,366 @@
+"""Layers on device tensors: the dense layer, layer norm and the 8-bit form of activations, each with its gradients.
+
+A ``VariationalAutoEncoder`` or ``AutoEncoder`` trains and runs a whole net behind one handle.  These are the layers by
+themselves, for nets that are put together from them: a deeper classifier on a balanced set, residual blocks between an
+encoder's layers, several classes' decoders over one batch.  In the reference a layer exists only inside its TensorFlow
+graph (smrt/autoencode/layer.py:348-464).
+
+    y = act(x W + b) + r        dense, dense_backward                    (activations and weight layout as in the estimators)
+    the same, a weight a class  dense_grouped, dense_grouped_backward    (rows sorted by class)
+    y = layer norm of x         layer_norm, layer_norm_backward
+    activations in 8 bits       pack_rows, unpack_rows, PackedRows       (what the backward calls take in a tensor's place)
+
+Tensors are ``float32``, ``bfloat16`` or ``float16`` on one GPU, 2-d, with a row's elements next to each other (rows may
+be any distance apart); sums are fp32.  Work is queued on the device's current torch stream and nothing waits for it, so the calls
+can be captured into graphs.  They take no part in torch's autograd -- the gradients are calls of their own -- and
+refuse a tensor that requires grad while grad mode is on.  There is no CPU fallback.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from .. import _hip
+
+__all__ = ["dense", "dense_backward", "dense_grouped", "dense_grouped_backward", "layer_norm", "layer_norm_backward",
+           "pack_rows", "unpack_rows", "PackedRows"]
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_BLOCK = 32                                      # columns that share a scale byte
+
+
+def _tensor(t, name, dim, dtype=None, device=None):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch tensor, got %s" % (name, type(t).__name__))
+    if t.dim() != dim:
+        raise ValueError("%s must have %d dimension(s), got shape %r" % (name, dim, tuple(t.shape)))
+    if dtype is None:
+        if t.dtype not in _DTYPES:
+            raise ValueError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+    elif t.dtype != dtype:
+        raise ValueError("%s must be %s, got %s" % (name, dtype, t.dtype))
+    if device is not None and t.device != device:
+        raise ValueError("%s is on %s, expected %s" % (name, t.device, device))
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s requires grad, and the layer calls take no part in autograd: detach it, or call under torch.no_grad()" % name)
+    if dim and t.shape[-1] > 1 and t.stride(-1) != 1 and t.numel():
+        raise ValueError("the elements of a row of %s must lie next to each other (strides %r)" % (name, t.stride()))
+    return t
+
+
+def _ld(t, name="matrix"):
+    """Leading dimension of a matrix (of the last two dimensions)."""
+    rows, cols = t.shape[-2:]
+    if rows <= 1 or cols == 0:
+        return max(cols, 1)
+    ld = t.stride(-2)
+    if ld < cols:
+        raise ValueError("the rows of %s overlap (strides %r)" % (name, t.stride()))
+    return ld
+
+
+def _shape(t, name, shape):
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("%s must have shape %r, got %r" % (name, tuple(shape), tuple(t.shape)))
+
+
+def _on_gpu(t):
+    if not t.is_cuda:
+        raise _hip.HipLibraryError("the layer calls run on an MI355X; there is no CPU fallback (got a tensor on %s)" % t.device)
+
+
+def _call(device, fn, what, *args):
+    """``fn(*args, stream)`` on the device's current stream, with that device current."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    if rc:
+        raise _hip.HipLibraryError("%s failed (%d): %s" % (what, rc, _hip.load().smrt_last_error().decode()))
+
+
+def _activation(name):
+    try:
+        return _hip.ACTIVATION_IDS[name]
+    except (KeyError, TypeError):
+        raise ValueError("activation must be one of %r, got %r" % (sorted(_hip.ACTIVATION_IDS), name)) from None
+
+
+# ------------------------------------------------------------------------------------------------ 8-bit form
+class PackedRows(object):
+    """A matrix of activations held in 8 bits: what a backward pass reads in place of the tensor it was made from.
+
+    ``q`` int8 ``[rows, cols rounded up to 32]``, ``scale`` uint8 ``[rows, cols / 32]``: 32 columns of a row share a power of two,
+    a value is ``q * 2 ** (scale - 127)`` with ``|q| <= 127`` -- off by at most 1/126 of the block's largest magnitude (half a step of
+    ``q``, of which that magnitude takes 63.5 or more).  A block that held an infinity or a NaN stands for 32 NaNs (scale 255).
+    ``dtype`` is the type of the values."""
+
+    __slots__ = ("q", "scale", "cols", "dtype")
+
+    def __init__(self, q, scale, cols, dtype):
+        cols = int(cols)
+        if dtype not in _DTYPES:
+            raise ValueError("dtype must be float32, bfloat16 or float16, got %s" % dtype)
+        _tensor(q, "q", 2, torch.int8)
+        _tensor(scale, "scale", 2, torch.uint8, q.device)
+        blocks = -(-cols // _BLOCK)
+        _shape(q, "q", (q.shape[0], blocks * _BLOCK))
+        _shape(scale, "scale", (q.shape[0], blocks))
+        self.q, self.scale, self.cols, self.dtype = q, scale, cols, dtype
+
+    @property
+    def shape(self):
+        return (self.q.shape[0], self.cols)
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def __repr__(self):
+        return "PackedRows(shape=%r, dtype=%s, device=%s)" % (self.shape, self.dtype, self.q.device)
+
+
+def _new_packed(rows, cols, dtype, device):
+    blocks = -(-cols // _BLOCK)
+    p = object.__new__(PackedRows)
+    p.q = torch.empty((rows, blocks * _BLOCK), dtype=torch.int8, device=device)
+    p.scale = torch.empty((rows, blocks), dtype=torch.uint8, device=device)
+    p.cols, p.dtype = cols, dtype
+    return p
+
+
+def pack_rows(x):
+    """The 8-bit form of ``x`` ``[rows, cols]`` (``PackedRows``)."""
+    _tensor(x, "x", 2)
+    ld = _ld(x, "x")
+    _on_gpu(x)
+    rows, cols = x.shape
+    p = _new_packed(rows, cols, x.dtype, x.device)
+    _call(x.device, _hip.load().smrt_pack_rows, "smrt_pack_rows", _DTYPES[x.dtype], x.data_ptr(), ld, rows, cols, p.q.data_ptr(), p.q.shape[1],
+          p.scale.data_ptr(), p.scale.shape[1])
+    return p
+
+
+def unpack_rows(packed):
+    """The values that ``packed`` stands for, a tensor ``[rows, cols]`` of ``packed.dtype``."""
+    if not isinstance(packed, PackedRows):
+        raise TypeError("packed must be PackedRows, got %s" % type(packed).__name__)
+    _on_gpu(packed.q)
+    rows, cols = packed.shape
+    out = torch.empty((rows, cols), dtype=packed.dtype, device=packed.device)
+    _call(packed.device, _hip.load().smrt_unpack_rows, "smrt_unpack_rows", _DTYPES[packed.dtype], packed.q.data_ptr(), _ld(packed.q, "q"),
+          packed.scale.data_ptr(), _ld(packed.scale, "scale"), rows, cols, out.data_ptr(), max(cols, 1))
+    return out
+
+
+def _kept(t, name, shape, dtype, device):
+    """A tensor or PackedRows of an earlier pass: ``(pointer, ld, scale pointer, scale ld)``."""
+    if isinstance(t, PackedRows):
+        if t.dtype != dtype or t.shape != tuple(shape) or t.device != device:
+            raise ValueError("%s must be a %s matrix of shape %r on %s, got %r" % (name, dtype, tuple(shape), device, t))
+        return t.q.data_ptr(), _ld(t.q, name), t.scale.data_ptr(), _ld(t.scale, name)
+    _tensor(t, name, 2, dtype, device)
+    _shape(t, name, shape)
+    return t.data_ptr(), _ld(t, name), None, 0
+
+
+# ------------------------------------------------------------------------------------------------ dense
+def _weights(weight, bias, x_dtype, device, k, ends):
+    """Checks of a weight ``[k, n]`` or ``[groups, k, n]``, its bias and the groups' ends: ``(n, groups, ldw, w_stride, bias_stride)``."""
+    grouped = ends is not None
+    _tensor(weight, "weight", 3 if grouped else 2, x_dtype, device)
+    if weight.shape[-2] != k:
+        raise ValueError("x has %d columns, weight has shape %r" % (k, tuple(weight.shape)))
+    n, groups = weight.shape[-1], weight.shape[0] if grouped else 1
+    ldw = _ld(weight, "weight")
+    w_stride = weight.stride(0) if grouped and groups > 1 else 0
+    if grouped:
+        _tensor(ends, "ends", 1, torch.int64, device)
+        _shape(ends, "ends", (groups,))
+        if not 1 <= groups <= 65535:
+            raise ValueError("between 1 and 65535 groups are supported, got %d" % groups)
+        if groups > 1 and w_stride < (k - 1) * ldw + n:
+            raise ValueError("the weights of the groups overlap (strides %r)" % (weight.stride(),))
+    bias_stride = n
+    if bias is not None:
+        _tensor(bias, "bias", 2 if grouped else 1, x_dtype, device)
+        _shape(bias, "bias", (groups, n) if grouped else (n,))
+        bias_stride = _ld(bias, "bias") if grouped else n
+    return n, groups, ldw, w_stride, bias_stride
+
+
+def _dense(x, ends, weight, bias, residual, activation, save, out):
+    act = _activation(activation)
+    if save not in (None, "activation", "packed"):
+        raise ValueError("save must be None, 'activation' or 'packed', got %r" % (save,))
+    _tensor(x, "x", 2)
+    dtype, device = x.dtype, x.device
+    rows, k = x.shape
+    n, groups, ldw, w_stride, bias_stride = _weights(weight, bias, dtype, device, k, ends)
+    ldx = _ld(x, "x")
+    r_ptr, ldr = None, 0
+    if residual is not None:
+        _tensor(residual, "residual", 2, dtype, device)
+        _shape(residual, "residual", (rows, n))
+        r_ptr, ldr = residual.data_ptr(), _ld(residual, "residual")
+    if out is not None:
+        _tensor(out, "out", 2, dtype, device)
+        _shape(out, "out", (rows, n))
+    _on_gpu(x)
+    y = torch.empty((rows, n), dtype=dtype, device=device) if out is None else out
+    saved, a_ptr, lda, s_ptr, lds = None, None, 0, None, 0
+    if save is not None and act != 1:                      # the identity's derivative needs nothing
+        if save == "packed":
+            saved = _new_packed(rows, n, dtype, device)
+            a_ptr, lda, s_ptr, lds = saved.q.data_ptr(), saved.q.shape[1], saved.scale.data_ptr(), saved.scale.shape[1]
+        elif residual is None:
+            saved = y
+        else:
+            saved = torch.empty((rows, n), dtype=dtype, device=device)
+            a_ptr, lda = saved.data_ptr(), n
+    args = _hip.Dense(_DTYPES[dtype], act, rows, k, n, groups, out is not None, None if ends is None else ends.data_ptr(),
+                      x.data_ptr(), ldx, None, 0, weight.data_ptr(), ldw, w_stride, None if bias is None else bias.data_ptr(), bias_stride,
+                      r_ptr, ldr, y.data_ptr(), _ld(y, "out"), a_ptr, lda, s_ptr, lds)
+    _call(device, _hip.load().smrt_dense_forward, "smrt_dense_forward", C.byref(args))
+    return y if save is None else (y, saved)
+
+
+def _dense_backward(grad, x, ends, weight, saved, activation, need_x, need_weight, need_bias):
+    act = _activation(activation)
+    _tensor(grad, "grad", 2)
+    dtype, device = grad.dtype, grad.device
+    k = weight.shape[-2] if isinstance(weight, torch.Tensor) and weight.dim() > 1 else 0
+    n, groups, ldw, w_stride, _ = _weights(weight, None, dtype, device, k, ends)
+    rows = grad.shape[0]
+    _shape(grad, "grad", (rows, n))
+    x_ptr, ldx, xs_ptr, ld_xs = _kept(x, "x", (rows, k), dtype, device)
+    a_ptr, lda, as_ptr, ld_as = None, 0, None, 0
+    if act != 1:
+        if saved is None:
+            raise ValueError("the gradient of %r needs what the forward pass saved" % activation)
+        a_ptr, lda, as_ptr, ld_as = _kept(saved, "saved", (rows, n), dtype, device)
+    ldg = _ld(grad, "grad")
+    _on_gpu(grad)
+    lead = () if ends is None else (groups,)
+    dx = torch.empty((rows, k), dtype=dtype, device=device) if need_x else None
+    dw = torch.empty(lead + (k, n), dtype=dtype, device=device) if need_weight else None
+    db = torch.empty(lead + (n,), dtype=dtype, device=device) if need_bias else None
+    args = _hip.Dense(_DTYPES[dtype], act, rows, k, n, groups, 0, None if ends is None else ends.data_ptr(),
+                      x_ptr, ldx, xs_ptr, ld_xs, weight.data_ptr(), ldw, w_stride, None, n, None, 0, None, 0, a_ptr, lda, as_ptr, ld_as,
+                      grad.data_ptr(), ldg, dx.data_ptr() if need_x else None, max(k, 1), dw.data_ptr() if need_weight else None, max(n, 1), k * n,
+                      db.data_ptr() if need_bias else None)
+    lib, ref = _hip.load(), C.byref(args)
+    size = lib.smrt_dense_backward_workspace(ref)
+    work = torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
+    _call(device, lib.smrt_dense_backward, "smrt_dense_backward", ref, None if work is None else work.data_ptr(), max(size, 0))
+    return dx, dw, db
+
+
+def dense(x, weight, bias=None, residual=None, activation="identity", save=None, out=None):
+    """``act(x @ weight + bias) + residual`` in one launch: ``x`` ``[rows, k]``, ``weight`` ``[k, n]`` (the estimators' layout).
+
+    ``save`` keeps what ``dense_backward`` needs, and makes the result ``(y, saved)``: ``"activation"`` the activation's value (``y`` itself
+    without a residual), ``"packed"`` its 8-bit form, written by the same launch.  For the identity, whose derivative needs
+    nothing, ``saved`` is None.  ``out`` receives ``y``; it may be the residual itself, and no other input."""
+    return _dense(x, None, weight, bias, residual, activation, save, out)
+
+
+def dense_backward(grad, x, weight, saved=None, activation="identity", need_x=True, need_weight=True, need_bias=True):
+    """Gradients ``(dx, dweight, dbias)`` of ``dense`` from ``grad`` = d loss / d y (None where not needed; the residual's gradient is ``grad``).
+
+    ``x`` and ``saved`` are the forward pass's tensors, or their 8-bit forms: the gradients are then those at the values the 8 bits
+    stand for."""
+    return _dense_backward(grad, x, None, weight, saved, activation, need_x, need_weight, need_bias)
+
+
+def dense_grouped(x, ends, weight, bias=None, residual=None, activation="identity", save=None, out=None):
+    """``dense`` with a weight for each class: rows ``[ends[g-1], ends[g])`` of ``x`` are multiplied by ``weight[g]`` (``[groups, k, n]``,
+    bias ``[groups, n]``), all classes in one launch.  ``ends`` is an int64 tensor on the device, the running sum of the classes' row counts;
+    classes may be empty.  An end below the one before it or past the rows counts as that bound.  Rows behind the last end are zero in a result
+    made here, and left as they were in ``out``."""
+    return _dense(x, _ends(ends), weight, bias, residual, activation, save, out)
+
+
+def dense_grouped_backward(grad, x, ends, weight, saved=None, activation="identity", need_x=True, need_weight=True, need_bias=True):
+    """Gradients ``(dx [rows, k], dweight [groups, k, n], dbias [groups, n])`` of ``dense_grouped``; zero for a class without rows, and
+    for rows that are in no class."""
+    return _dense_backward(grad, x, _ends(ends), weight, saved, activation, need_x, need_weight, need_bias)
+
+
+def _ends(ends):
+    if ends is None:
+        raise TypeError("ends must be a torch tensor, got NoneType")
+    return ends
+
+
+# ------------------------------------------------------------------------------------------------ layer norm
+def _norm_weight(weight, bias, dtype, device, n):
+    if weight is None:
+        if bias is not None:
+            raise ValueError("bias without weight is not supported")
+        return 0
+    if not isinstance(weight, torch.Tensor) or weight.dtype not in (dtype, torch.float32):
+        raise ValueError("weight must be a tensor of %s or float32" % dtype)
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _tensor(t, name, 1, weight.dtype, device)
+            _shape(t, name, (n,))
+    return int(weight.dtype == torch.float32)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
+    """``(y, mean, rstd)``: each row of ``x`` ``[rows, n]`` less its mean, over ``sqrt(variance + eps)``, times ``weight`` plus ``bias``
+    (``[n]``, of ``x``'s type or float32).  ``mean`` and ``rstd`` are float32 ``[rows]``, for the backward pass.  1 <= n <= 32768.
+    ``out`` receives ``y`` and may be ``x``."""
+    _tensor(x, "x", 2)
+    dtype, device = x.dtype, x.device
+    rows, n = x.shape
+    if not 1 <= n <= 32768:
+        raise ValueError("layer norm takes 1 to 32768 columns, got %d" % n)
+    if not eps >= 0.0:
+        raise ValueError("eps must be >= 0, got %r" % (eps,))
+    w_f32 = _norm_weight(weight, bias, dtype, device, n)
+    if out is not None:
+        _tensor(out, "out", 2, dtype, device)
+        _shape(out, "out", (rows, n))
+    ldx = _ld(x, "x")
+    _on_gpu(x)
+    y = torch.empty((rows, n), dtype=dtype, device=device) if out is None else out
+    stats = torch.empty((2, rows), dtype=torch.float32, device=device)
+    mean, rstd = stats.unbind(0)
+    args = _hip.LayerNorm(_DTYPES[dtype], w_f32, rows, n, eps, x.data_ptr(), ldx, None, 0, None if weight is None else weight.data_ptr(),
+                          None if bias is None else bias.data_ptr(), y.data_ptr(), _ld(y, "out"), mean.data_ptr(), rstd.data_ptr())
+    _call(device, _hip.load().smrt_layer_norm_forward, "smrt_layer_norm_forward", C.byref(args))
+    return y, mean, rstd
+
+
+def layer_norm_backward(grad, x, mean, rstd, weight=None, need_x=True, need_weight=True, need_bias=True):
+    """Gradients ``(dx, dweight, dbias)`` of ``layer_norm`` from ``grad`` = d loss / d y.  ``x`` is the forward pass's input or its 8-bit form;
+    ``mean`` and ``rstd`` are what it returned.  Without a ``weight`` only ``dx`` is computed."""
+    _tensor(grad, "grad", 2)
+    dtype, device = grad.dtype, grad.device
+    rows, n = grad.shape
+    if not 1 <= n <= 32768:
+        raise ValueError("layer norm takes 1 to 32768 columns, got %d" % n)
+    w_f32 = _norm_weight(weight, None, dtype, device, n)
+    x_ptr, ldx, xs_ptr, ld_xs = _kept(x, "x", (rows, n), dtype, device)
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        _tensor(t, name, 1, torch.float32, device)
+        _shape(t, name, (rows,))
+    need_weight, need_bias = need_weight and weight is not None, need_bias and weight is not None
+    ldg = _ld(grad, "grad")
+    _on_gpu(grad)
+    dx = torch.empty((rows, n), dtype=dtype, device=device) if need_x else None
+    dw = torch.empty((n,), dtype=weight.dtype, device=device) if need_weight else None
+    db = torch.empty((n,), dtype=weight.dtype, device=device) if need_bias else None
+    args = _hip.LayerNorm(_DTYPES[dtype], w_f32, rows, n, 0.0, x_ptr, ldx, xs_ptr, ld_xs, None if weight is None else weight.data_ptr(), None,
+                          None, 0, mean.data_ptr(), rstd.data_ptr(), grad.data_ptr(), ldg, dx.data_ptr() if need_x else None, n,
+                          dw.data_ptr() if need_weight else None, db.data_ptr() if need_bias else None)
+    lib, ref = _hip.load(), C.byref(args)
+    size = lib.smrt_layer_norm_backward_workspace(ref)
+    work = torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
+    _call(device, lib.smrt_layer_norm_backward, "smrt_layer_norm_backward", ref, None if work is None else work.data_ptr(), max(size, 0))
+    return dx, dw, db

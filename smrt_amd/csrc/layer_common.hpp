@@ -1,0 +1,190 @@
+// Shared by the layer operators (dense, layer norm, 8-bit checkpoints): element types, activations, groups of rows.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include "device_utils.hpp"
+
+namespace smrt {
+namespace layers {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int PACK_BLOCK = 32;            // columns of a row that share one scale byte of the 8-bit form
+
+// Rows move in pieces of 8 columns.  The tensors are a user's: rows may start at any element, so the pieces are read and
+// written as memory of the element's own alignment (global loads and stores take any address on gfx950; 16 bytes stay one
+// instruction).  A piece that the row's end cuts goes element by element.
+template <class T> struct alignas(sizeof(T)) Piece { T v[8]; };
+
+template <class T> __device__ __forceinline__ void load8(const T* __restrict__ p, int valid, T (&v)[8]) {
+    if (valid >= 8) {
+        __builtin_memcpy(v, p, 8 * sizeof(T));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < valid ? p[j] : (T)0.0f;
+    }
+}
+template <class T> __device__ __forceinline__ void store8(T* p, int valid, const T (&v)[8]) {
+    if (valid >= 8) {
+        __builtin_memcpy(p, v, 8 * sizeof(T));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) if (j < valid) p[j] = v[j];
+    }
+}
+template <class T> __device__ __forceinline__ void load8f(const T* __restrict__ p, int valid, float (&f)[8]) {
+    T v[8];
+    load8(p, valid, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (float)v[j];
+}
+template <class T> __device__ __forceinline__ void store8f(T* p, int valid, const float (&f)[8]) {
+    T v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (T)f[j];
+    store8(p, valid, v);
+}
+
+// Activations.  Unlike act_fwd these hand a NaN on (relu of the training kernels is fmaxf, which drops it: there the loss
+// reports it; here the value is the user's).
+__device__ __forceinline__ void layer_act8(int act, float (&v)[8]) {
+    switch (act) {
+        case ACT_SIGMOID:
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = fast_sigmoid(v[j]);
+            break;
+        case ACT_TANH:
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = tanhf(v[j]);
+            break;
+        case ACT_RELU:
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];
+            break;
+        case ACT_ELU:
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = v[j] > 0.0f ? v[j] : expm1f(v[j]);
+            break;
+        default: break;
+    }
+}
+// g := g * d act(z) / dz, from a = act(z); a NaN in a is handed on
+__device__ __forceinline__ void layer_act_grad8(int act, const float (&a)[8], float (&g)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float nan = a[j] != a[j] ? a[j] : 0.0f;
+        switch (act) {
+            case ACT_SIGMOID: g[j] *= a[j] * (1.0f - a[j]); break;
+            case ACT_TANH:    g[j] *= 1.0f - a[j] * a[j]; break;
+            case ACT_RELU:    g[j] = a[j] > 0.0f ? g[j] : nan; break;
+            case ACT_ELU:     g[j] = a[j] >= 0.0f ? g[j] : g[j] * (a[j] + 1.0f); break;
+            default:          break;
+        }
+    }
+}
+
+// ---- the 8-bit form.  32 columns of a row share 2^e; a value is a whole number q in [-127, 127] times 2^e, e the smallest
+// exponent with max|x| <= 127 * 2^e.  q * 2^e has 7 significant bits: EXACT in bf16 (and, with e >= -24, in f16), so what the
+// backward products read is the value itself, with no second rounding.  The scale byte is e + 127; 255 marks a block that
+// held an infinity or a NaN: all its values stand for NaN.
+template <class T> struct PackRange { static constexpr int lo = -126, hi = 122; };      // 64 * 2^122 is 2^128
+template <> struct PackRange<f16> { static constexpr int lo = -24, hi = 10; };          // 64 * 2^10 is 2^16
+// scale byte for the largest magnitude of a block (given as the bits of |x|, where NaN is above infinity above all numbers)
+template <class T> __device__ __forceinline__ int pack_scale(uint32_t top_bits) {
+    if (top_bits >= 0x7f800000u) return 255;
+    int e = (int)(top_bits >> 23) - 127 - 6;                                  // top in [64, 128) * 2^e
+    if ((top_bits & 0x7fffffu) > 0x7e0000u) ++e;                              // over 127 * 2^e
+    return (e < PackRange<T>::lo ? PackRange<T>::lo : e) + 127;
+}
+template <class T> __device__ __forceinline__ int pack_value(float x, int byte) {
+    if (byte == 255) return 0;
+    const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);          // 2^-e, a normal number for e in [-126, 122]
+    const float q = __builtin_rintf(x * inv);
+    const float lim = byte == PackRange<T>::hi + 127 ? 63.0f : 127.0f;        // 64 * 2^hi would be an infinity of T
+    return (int)fminf(fmaxf(q, -lim), lim);
+}
+__device__ __forceinline__ float unpack_scale(int byte) {
+    return byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)byte << 23);
+}
+__device__ __forceinline__ void unpack8(u32x2 q, float scale, float (&f)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (float)((int)(q[j / 4] << (24 - 8 * (j % 4))) >> 24) * scale;
+}
+// Four neighbouring lanes hold a block (8 columns each; columns behind the row's end are zero): writes its 8 bytes of q and,
+// from the first of the four, the scale byte.
+template <class T> __device__ __forceinline__ void pack_block(const float (&f)[8], int lane, bool store, int8_t* q, uint8_t* scale) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { const uint32_t b = __float_as_uint(f[j]) & 0x7fffffffu; top = top > b ? top : b; }
+#pragma unroll
+    for (int d = 1; d <= 2; d <<= 1) { const uint32_t o = (uint32_t)__shfl_xor((int)top, d); top = top > o ? top : o; }
+    const int byte = pack_scale<T>(top);
+    u32x2 w = {0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j / 4] |= ((uint32_t)pack_value<T>(f[j], byte) & 255u) << (8 * (j % 4));
+    if (store) {
+        __builtin_memcpy(q, &w, 8);
+        if ((lane & 3) == 0) *scale = (uint8_t)byte;
+    }
+}
+
+// ---- groups of rows.  ends[g] is where group g's rows end (it begins where g - 1 ends, group 0 at row 0).  The array is
+// device memory that the host never sees, so every kernel makes it sound for itself: an end is clamped to [0, rows] and
+// never lies before an earlier one.  Whatever the array holds, groups are then disjoint and inside the matrix.
+// All 64 lanes of a wave call these together; the results are the same in all lanes.
+struct RowSpan { int group; int r0, r1; };      // group -1: rows that no group has; r0 >= r1: nothing
+
+__device__ __forceinline__ int clamp_end(const int64_t* __restrict__ ends, int g, int n_groups, int rows) {
+    if (g >= n_groups) return 0;
+    const int64_t e = ends[g];
+    return e < 0 ? 0 : e > rows ? rows : (int)e;
+}
+// rows of group g
+__device__ __forceinline__ RowSpan group_rows(const int64_t* __restrict__ ends, int g, int rows) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int i = lane; i < g; i += 64) { const int e = clamp_end(ends, i, g, rows); before = e > before ? e : before; }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) { const int o = __shfl_xor(before, d); before = o > before ? o : before; }
+    const int e = clamp_end(ends, g, g + 1, rows);
+    return {g, before, e > before ? e : before};
+}
+// the t-th tile of `tile` rows, where no tile crosses from one group into the next; behind the last group come the rows
+// that no group has
+__device__ __forceinline__ RowSpan tile_rows(const int64_t* __restrict__ ends, int n_groups, int rows, int t, int tile) {
+    const int lane = threadIdx.x & 63;
+    int end0 = 0, tiles0 = 0;
+    for (int base = 0; base < n_groups; base += 64) {
+        int e = clamp_end(ends, base + lane, n_groups, rows);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(e, d); if (lane >= d && o > e) e = o; }
+        e = e > end0 ? e : end0;
+        int prev = __shfl_up(e, 1);
+        if (lane == 0) prev = end0;
+        const int own = (e - prev + tile - 1) / tile;
+        int sum = own;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(sum, d); if (lane >= d) sum += o; }
+        sum += tiles0;
+        const unsigned long long hit = __ballot(t < sum);
+        if (hit) {
+            const int f = __builtin_ctzll(hit);
+            const int first = __shfl(sum - own, f), begin = __shfl(prev, f), end = __shfl(e, f);
+            return {base + f, begin + (t - first) * tile, end};
+        }
+        end0 = __shfl(e, 63);
+        tiles0 = __shfl(sum, 63);
+    }
+    const long r0 = (long)end0 + (long)(t - tiles0) * tile;
+    return {-1, r0 < rows ? (int)r0 : rows, rows};
+}
+
+}  // namespace layers
+}  // namespace smrt

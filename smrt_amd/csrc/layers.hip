@@ -1,0 +1,613 @@
+// The layer operators of the C ABI (include/smrt_hip.h: smrt_dense_*, smrt_layer_norm_*, smrt_pack_rows, smrt_unpack_rows):
+// argument checks, workspaces, launches, and the kernels beside the products (layer_gemm.hpp).
+#include <algorithm>
+#include <string>
+#include "layers.hpp"
+#include "../../include/smrt_hip.h"
+
+int smrt_set_error(int code, const std::string& m);      // api.hip: the thread's error text
+
+namespace smrt {
+namespace layers {
+namespace {
+
+constexpr int64_t MAX_ROWS = 0x7fffffff - 4096, MAX_COLS = 1 << 30;
+constexpr int MAX_GROUPS = 65535;
+
+// ------------------------------------------------------------------------------------------------ dz = g * act'(a), column sums
+// One pass over g (and a): writes dz for the two products that read it, and sums its columns into db on the way (in fp32, from
+// the values before they are rounded to T).  256 columns x 8 rows per workgroup step; a workgroup owns a slice of one group's rows.
+struct DzArgs {
+    const void* grad; int64_t ldg;
+    const void* a; int64_t lda; const uint8_t* a_scale; int64_t ld_a_scale;
+    void* dz; int64_t ld_dz;                       // null: the identity, whose dz is g
+    float* part;                                   // [slices][groups][n], or null where slices == 1
+    void* db; int64_t db_stride;                   // null: not wanted
+    const int64_t* ends; int32_t groups, rows, n, slices, act, col_blocks;
+};
+
+template <class T, bool PACKED> __global__ void __launch_bounds__(256) dz_kernel(DzArgs p) {
+    __shared__ float sums[8][256];
+    int bid = blockIdx.x;
+    const int cb = bid % p.col_blocks;
+    bid /= p.col_blocks;
+    const int group = bid % p.groups, slice = bid / p.groups;
+    int r0 = 0, r1 = p.rows;
+    if (p.ends) { const RowSpan s = group_rows(p.ends, group, p.rows); r0 = s.r0; r1 = s.r1; }
+    const int per = (r1 - r0 + p.slices - 1) / p.slices;
+    const long first = r0 + (long)slice * per;
+    const int lo = first < r1 ? (int)first : r1, hi = r1 - lo > per ? lo + per : r1;
+    const int col = cb * 256 + (threadIdx.x & 31) * 8, valid = p.n - col;
+    float sum[8] = {};
+    if (valid > 0) {
+        for (int row = lo + (threadIdx.x >> 5); row < hi; row += 8) {
+            float g[8];
+            load8f((const T*)p.grad + (int64_t)row * p.ldg + col, valid, g);
+            if (p.dz) {
+                float a[8];
+                if constexpr (PACKED) {
+                    u32x2 q;
+                    __builtin_memcpy(&q, (const int8_t*)p.a + (int64_t)row * p.lda + col, 8);
+                    unpack8(q, unpack_scale(p.a_scale[(int64_t)row * p.ld_a_scale + col / PACK_BLOCK]), a);
+                } else {
+                    load8f((const T*)p.a + (int64_t)row * p.lda + col, valid, a);
+                }
+                layer_act_grad8(p.act, a, g);
+                store8f((T*)p.dz + (int64_t)row * p.ld_dz + col, valid, g);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[j] += g[j];
+        }
+    }
+    if (!p.db) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sums[threadIdx.x >> 5][(threadIdx.x & 31) * 8 + j] = sum[j];
+    __syncthreads();
+    const int c = cb * 256 + threadIdx.x;
+    if (c < p.n) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += sums[i][threadIdx.x];
+        if (p.part) p.part[((int64_t)slice * p.groups + group) * p.n + c] = s;
+        else ((T*)p.db)[(int64_t)group * p.db_stride + c] = (T)s;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ joining of partial sums
+// out[row][col] = sum over slabs of slab[s][row][col], in the order of s: the result does not depend on timing.
+struct JoinPart {                     // blocks == 0: nothing
+    const float* slab; int64_t slabs, rows, cols, slab_stride;     // slab s at s * slab_stride
+    void* out; int64_t ld, group_rows, group_stride;               // row r of out: (r / group_rows) * group_stride + (r % group_rows) * ld
+    int32_t out_f32;
+    int32_t blocks;
+};
+// SL threads share the slabs of a piece of 8 columns: many for the long sums over workgroups, one for the few splits of a product
+template <class T, int SL> __device__ __forceinline__ void join(const JoinPart& p, int block, float (*lds)[8]) {
+    constexpr int PIECES = 256 / SL;
+    const int64_t per_row = (p.cols + 7) / 8;
+    const int sl = threadIdx.x / PIECES;
+    const int64_t piece = (int64_t)block * PIECES + threadIdx.x % PIECES;
+    const int64_t row = piece / per_row, col = (piece % per_row) * 8;
+    const int valid = row < p.rows ? (int)(p.cols - col < 8 ? p.cols - col : 8) : 0;
+    float sum[8] = {};
+    if (valid > 0) {
+        const float* src = p.slab + row * p.cols + col;
+#pragma unroll 4
+        for (int64_t s = sl; s < p.slabs; s += SL) {
+            float v[8];
+            load8f(src + s * p.slab_stride, valid, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[j] += v[j];
+        }
+    }
+    if constexpr (SL > 1) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) lds[threadIdx.x][j] = sum[j];
+        __syncthreads();
+        if (sl) return;
+        for (int i = 1; i < SL; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[j] += lds[i * PIECES + threadIdx.x][j];
+    }
+    if (valid <= 0) return;
+    const int64_t at = (row / p.group_rows) * p.group_stride + (row % p.group_rows) * p.ld + col;
+    if (p.out_f32) store8((float*)p.out + at, valid, sum);
+    else store8f((T*)p.out + at, valid, sum);
+}
+template <class T, int SL0, int SL1> __global__ void __launch_bounds__(256) join_kernel(JoinPart a, JoinPart b) {
+    __shared__ float lds[256][8];
+    if ((int)blockIdx.x < a.blocks) join<T, SL0>(a, blockIdx.x, lds);
+    else join<T, SL1>(b, blockIdx.x - a.blocks, lds);
+}
+JoinPart join_part(const float* slab, int64_t slabs, int64_t slab_stride, int64_t rows, int64_t cols, void* out, int64_t ld, int64_t group_rows, int64_t group_stride,
+                   bool out_f32, int sl) {
+    const int64_t pieces = rows * ((cols + 7) / 8), per = 256 / sl;
+    return {slab, slabs, rows, cols, slab_stride, out, ld, std::max<int64_t>(group_rows, 1), group_stride, out_f32, (int32_t)((pieces + per - 1) / per)};
+}
+
+// ------------------------------------------------------------------------------------------------ layer norm
+// A row lives in the registers of TPR lanes (8 columns each, CH times): one read, the mean, then the squares of the differences
+// from it.  Rows go round the workgroups, so a lane keeps its columns: weight and bias are read once, and in the backward
+// pass the sums of their gradients stay in registers until the end.
+struct NormArgs {
+    const void* x; int64_t ldx; const uint8_t* x_scale; int64_t ld_x_scale;
+    const void* weight; const void* bias; int32_t w_f32;
+    void* y; int64_t ldy; float* mean; float* rstd;
+    const void* grad; int64_t ldg; void* dx; int64_t lddx; void* dw; void* db; float* part;
+    int32_t rows, n; float eps;
+};
+
+template <int TPR> struct RowSum {
+    // sum over the TPR lanes of a row; with more than a wave, all threads of the workgroup take part
+    __device__ static __forceinline__ float sum(float v, float* lds) {
+#pragma unroll
+        for (int d = (TPR < 64 ? TPR : 64) / 2; d; d >>= 1) v += __shfl_xor(v, d);
+        if constexpr (TPR > 64) {
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+            __syncthreads();
+            v = 0.0f;
+#pragma unroll
+            for (int i = 0; i < TPR / 64; ++i) v += lds[i];
+        }
+        return v;
+    }
+};
+template <class T> __device__ __forceinline__ void load_weight(const void* p, int w_f32, int col, int valid, float fill, float (&w)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = fill;
+    if (!p || valid <= 0) return;
+    if (w_f32) load8f((const float*)p + col, valid, w);
+    else load8f((const T*)p + col, valid, w);
+}
+
+template <class T, int TPR, int CH>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_forward_kernel(NormArgs p) {
+    constexpr int THREADS = TPR > 256 ? TPR : 256, ROWS = THREADS / TPR;
+    __shared__ float lds[16];
+    const int lane = threadIdx.x % TPR;
+    float w[CH][8], b[CH][8];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int col = (c * TPR + lane) * 8;
+        load_weight<T>(p.weight, p.w_f32, col, p.n - col, 1.0f, w[c]);
+        load_weight<T>(p.bias, p.w_f32, col, p.n - col, 0.0f, b[c]);
+    }
+    const float inv_n = 1.0f / (float)p.n;
+    for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < p.rows; row0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t row = row0 + threadIdx.x / TPR;
+        const bool live = row < p.rows;
+        float x[CH][8], sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int col = (c * TPR + lane) * 8;
+            load8f((const T*)p.x + row * p.ldx + col, live ? p.n - col : 0, x[c]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += x[c][j];
+        }
+        const float mean = RowSum<TPR>::sum(sum, lds) * inv_n;
+        float sq = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int valid = p.n - (c * TPR + lane) * 8;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { x[c][j] -= mean; sq += j < valid ? x[c][j] * x[c][j] : 0.0f; }
+        }
+        const float rstd = 1.0f / sqrtf(RowSum<TPR>::sum(sq, lds) * inv_n + p.eps);
+        if (!live) continue;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int col = (c * TPR + lane) * 8;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[c][j] = x[c][j] * rstd * w[c][j] + b[c][j];
+            if (p.n - col > 0) store8f((T*)p.y + row * p.ldy + col, p.n - col, x[c]);
+        }
+        if (lane == 0) { p.mean[row] = mean; p.rstd[row] = rstd; }
+    }
+}
+
+template <class T, bool PACKED, int TPR, int CH>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_backward_kernel(NormArgs p) {
+    constexpr int THREADS = TPR > 256 ? TPR : 256, ROWS = THREADS / TPR;
+    __shared__ float lds[16];
+    __shared__ float sums[ROWS > 1 ? ROWS : 1][TPR <= 64 ? TPR * 8 : 1];
+    const int lane = threadIdx.x % TPR;
+    float w[CH][8], dw[CH][8] = {}, db[CH][8] = {};
+#pragma unroll
+    for (int c = 0; c < CH; ++c) { const int col = (c * TPR + lane) * 8; load_weight<T>(p.weight, p.w_f32, col, p.n - col, 1.0f, w[c]); }
+    const float inv_n = 1.0f / (float)p.n;
+    for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < p.rows; row0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t row = row0 + threadIdx.x / TPR;
+        const bool live = row < p.rows;
+        const float mean = live ? p.mean[row] : 0.0f, rstd = live ? p.rstd[row] : 0.0f;
+        float h[CH][8], g[CH][8], s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int col = (c * TPR + lane) * 8, valid = live ? p.n - col : 0;
+            load8f((const T*)p.grad + row * p.ldg + col, valid, g[c]);
+            if constexpr (PACKED) {
+                u32x2 q = {0u, 0u};
+                float scale = 0.0f;
+                if (valid > 0) {
+                    __builtin_memcpy(&q, (const int8_t*)p.x + row * p.ldx + col, 8);
+                    scale = unpack_scale(p.x_scale[row * p.ld_x_scale + col / PACK_BLOCK]);
+                }
+                unpack8(q, scale, h[c]);
+            } else {
+                load8f((const T*)p.x + row * p.ldx + col, valid, h[c]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int valid = live ? p.n - (c * TPR + lane) * 8 : 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                h[c][j] = j < valid ? (h[c][j] - mean) * rstd : 0.0f;
+                dw[c][j] += g[c][j] * h[c][j];
+                db[c][j] += g[c][j];
+                g[c][j] *= w[c][j];
+                s1 += g[c][j];
+                s2 += g[c][j] * h[c][j];
+            }
+        }
+        s1 = RowSum<TPR>::sum(s1, lds) * inv_n;
+        s2 = RowSum<TPR>::sum(s2, lds) * inv_n;
+        if (!live || !p.dx) continue;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int col = (c * TPR + lane) * 8;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g[c][j] = rstd * (g[c][j] - s1 - h[c][j] * s2);
+            if (p.n - col > 0) store8f((T*)p.dx + row * p.lddx + col, p.n - col, g[c]);
+        }
+    }
+    // this workgroup's share of the weight's and the bias's gradient: to `part` [workgroups][2][n], or out at once where it is the only one
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        void* out = which ? p.db : p.dw;
+        if (!out) continue;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int col = (c * TPR + lane) * 8, valid = p.n - col;
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = which ? db[c][j] : dw[c][j];
+            if constexpr (ROWS > 1) {
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sums[threadIdx.x / TPR][lane * 8 + j] = v[j];
+                __syncthreads();
+                if (threadIdx.x >= TPR) continue;
+                for (int i = 1; i < ROWS; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] += sums[i][lane * 8 + j];
+            }
+            if (valid <= 0) continue;
+            if (p.part) store8(p.part + ((int64_t)blockIdx.x * 2 + which) * p.n + col, valid, v);
+            else if (p.w_f32) store8((float*)out + col, valid, v);
+            else store8f((T*)out + col, valid, v);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ the 8-bit form on its own
+struct PackArgs { const void* x; int64_t ldx; int8_t* q; int64_t ldq; uint8_t* scale; int64_t ld_scale; int64_t rows; int32_t n; void* out; };
+
+template <class T> __global__ void __launch_bounds__(256) pack_kernel(PackArgs p) {
+    const int64_t per_row = (int64_t)((p.n + PACK_BLOCK - 1) / PACK_BLOCK) * 4, total = p.rows * per_row;       // whole blocks: four lanes
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {      // stay together
+        const int64_t row = i / per_row;
+        const int col = (int)(i % per_row) * 8;
+        float f[8];
+        load8f((const T*)p.x + row * p.ldx + col, p.n - col, f);
+        pack_block<T>(f, (int)(i & 3), true, p.q + row * p.ldq + col, p.scale + row * p.ld_scale + col / PACK_BLOCK);
+    }
+}
+template <class T> __global__ void __launch_bounds__(256) unpack_kernel(PackArgs p) {
+    const int64_t per_row = (p.n + 7) / 8, total = p.rows * per_row;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / per_row;
+        const int col = (int)(i % per_row) * 8;
+        u32x2 q;
+        __builtin_memcpy(&q, p.q + row * p.ldq + col, 8);
+        float f[8];
+        unpack8(q, unpack_scale(p.scale[row * p.ld_scale + col / PACK_BLOCK]), f);
+        store8f((T*)p.out + row * p.ldx + col, p.n - col, f);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+int fail(const char* who, const char* what) { return smrt_set_error(-1, std::string(who) + ": " + what); }
+int launched(const char* who, hipError_t e) { return e == hipSuccess ? 0 : smrt_set_error(-2, std::string(who) + ": " + hipGetErrorString(e)); }
+int elem_size(int dtype) { return dtype == SMRT_F32 ? 4 : 2; }
+int64_t pad(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+}
+int64_t span(int64_t rows, int64_t ld, int64_t cols) { return rows > 0 ? (rows - 1) * ld + cols : 0; }
+
+int check_dense(const smrt_dense* p, const char* who) {
+    if (!p) return fail(who, "null argument");
+    if (p->dtype < 0 || p->dtype > SMRT_F16) return fail(who, "dtype must be SMRT_F32, SMRT_BF16 or SMRT_F16");
+    if (p->activation < 0 || p->activation > SMRT_ACT_TANH) return fail(who, "bad activation id");
+    if (p->rows < 0 || p->rows > MAX_ROWS || p->k < 0 || p->k > MAX_COLS || p->n < 0 || p->n > MAX_COLS) return fail(who, "bad sizes");
+    if (p->groups < 1 || p->groups > MAX_GROUPS) return fail(who, "groups must be in [1, 65535]");
+    if (p->groups > 1 && !p->ends) return fail(who, "more than one group needs ends");
+    if (p->ldx < p->k || p->ldw < p->n) return fail(who, "a leading dimension is below its columns");
+    if (p->groups > 1 && p->w_stride < span(p->k, p->ldw, p->n)) return fail(who, "the groups' weights overlap");
+    if (p->w_stride < 0) return fail(who, "bad sizes");
+    if (p->groups > 1 && (p->bias || p->db) && p->bias_stride < p->n) return fail(who, "the groups' biases overlap");
+    const bool product = p->rows && p->n && p->k;
+    if (product && (!p->x || !p->w)) return fail(who, "null pointer");
+    return 0;
+}
+
+hipError_t gemm(int dtype, int layout, const GemmArgs& g, hipStream_t s) {
+    return dtype == SMRT_F32 ? layer_gemm_f32(layout, g, s) : dtype == SMRT_BF16 ? layer_gemm_bf16(layout, g, s) : layer_gemm_f16(layout, g, s);
+}
+
+struct BackwardPlan {
+    bool need_dz, need_sum;
+    int dz_slices, splits;
+    int64_t ld_dz, dz_bytes, slab_off, slab_bytes, part_off, part_bytes, total;
+};
+BackwardPlan plan_backward(const smrt_dense* p) {
+    BackwardPlan b = {};
+    const int64_t es = elem_size(p->dtype), G = p->groups;
+    b.need_dz = p->activation != SMRT_ACT_IDENTITY && (p->dx || p->dw || p->db);
+    b.need_sum = p->db != nullptr;
+    b.ld_dz = pad(p->n, 8);
+    b.dz_bytes = b.need_dz ? pad(p->rows * b.ld_dz * es, 256) : 0;
+    const int64_t col_blocks = (p->n + 255) / 256, avg = p->rows / G;
+    // slices of a group's rows: enough workgroups for every CU several times over, none with fewer than 64 rows
+    b.dz_slices = (int)std::max<int64_t>(1, std::min<int64_t>(avg / 64, 2048 / std::max<int64_t>(1, col_blocks * G)));
+    b.part_bytes = b.need_sum && b.dz_slices > 1 ? pad((int64_t)b.dz_slices * G * p->n * 4, 256) : 0;
+    const int64_t tiles = ((p->k + 127) / 128) * ((p->n + 127) / 128) * G;
+    b.splits = p->dw ? (int)std::max<int64_t>(1, std::min<int64_t>(avg / 512, 512 / std::max<int64_t>(1, tiles))) : 1;
+    b.slab_bytes = p->dw && b.splits > 1 ? pad((int64_t)b.splits * G * p->k * p->n * 4, 256) : 0;
+    b.slab_off = b.dz_bytes;
+    b.part_off = b.slab_off + b.slab_bytes;
+    b.total = b.part_off + b.part_bytes;
+    return b;
+}
+
+template <class F> hipError_t by_type(int dtype, F f) {
+    return dtype == SMRT_F32 ? f((float)0) : dtype == SMRT_BF16 ? f((bf16)0.0f) : f((f16)0.0f);
+}
+
+template <class T> hipError_t launch_dz(const DzArgs& d, hipStream_t s) {
+    const unsigned blocks = (unsigned)((int64_t)d.col_blocks * d.groups * d.slices);
+    if (d.a_scale) hipLaunchKernelGGL((dz_kernel<T, true>), dim3(blocks), dim3(256), 0, s, d);
+    else hipLaunchKernelGGL((dz_kernel<T, false>), dim3(blocks), dim3(256), 0, s, d);
+    return hipGetLastError();
+}
+
+int norm_blocks(int64_t rows, int rows_per_block, int most) { return (int)std::max<int64_t>(1, std::min<int64_t>((rows + rows_per_block - 1) / rows_per_block, most)); }
+constexpr int NORM_MAX_COLS = 1024 * 8 * 4;
+// lanes of a row and pieces of a lane, by the row's width
+template <class F> hipError_t by_width(int64_t n, F f) {
+    if (n <= 64) return f(std::integral_constant<int, 8>(), std::integral_constant<int, 1>());
+    if (n <= 128) return f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
+    if (n <= 256) return f(std::integral_constant<int, 32>(), std::integral_constant<int, 1>());
+    if (n <= 512) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+    if (n <= 1024) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+    if (n <= 2048) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
+    if (n <= 4096) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
+    if (n <= 8192) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
+    if (n <= 16384) return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
+    return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
+}
+int norm_rows_per_block(int64_t n) { return n <= 64 ? 32 : n <= 128 ? 16 : n <= 256 ? 8 : n <= 1024 ? 4 : 1; }
+int norm_backward_blocks(int64_t rows, int64_t n) { return norm_blocks(rows, norm_rows_per_block(n), 512); }
+
+int check_norm(const smrt_layer_norm* p, const char* who) {
+    if (!p) return fail(who, "null argument");
+    if (p->dtype < 0 || p->dtype > SMRT_F16) return fail(who, "dtype must be SMRT_F32, SMRT_BF16 or SMRT_F16");
+    if (p->rows < 0 || p->rows > MAX_ROWS) return fail(who, "bad sizes");
+    if (p->n < 1 || p->n > NORM_MAX_COLS) return fail(who, "n must be in [1, 32768]");
+    if (p->ldx < p->n) return fail(who, "a leading dimension is below its columns");
+    if (p->rows && (!p->x || !p->mean || !p->rstd)) return fail(who, "null pointer");
+    return 0;
+}
+NormArgs norm_args(const smrt_layer_norm* p) {
+    NormArgs a = {};
+    a.x = p->x; a.ldx = p->ldx; a.x_scale = p->x_scale; a.ld_x_scale = p->ld_x_scale;
+    a.weight = p->weight; a.bias = p->bias; a.w_f32 = p->weight_f32 || p->dtype == SMRT_F32;
+    a.y = p->y; a.ldy = p->ldy; a.mean = p->mean; a.rstd = p->rstd;
+    a.grad = p->grad; a.ldg = p->ldg; a.dx = p->dx; a.lddx = p->lddx; a.dw = p->dw; a.db = p->db;
+    a.rows = (int32_t)p->rows; a.n = (int32_t)p->n; a.eps = p->eps;
+    return a;
+}
+
+int check_pack(const char* who, int dtype, const void* x, int64_t ldx, int64_t rows, int64_t n, const void* q, int64_t ldq, const void* scale, int64_t ld_scale) {
+    if (dtype < 0 || dtype > SMRT_F16) return fail(who, "dtype must be SMRT_F32, SMRT_BF16 or SMRT_F16");
+    if (rows < 0 || rows > MAX_ROWS || n < 0 || n > MAX_COLS) return fail(who, "bad sizes");
+    if (ldx < n || ldq < pad(n, PACK_BLOCK) || ld_scale < (n + PACK_BLOCK - 1) / PACK_BLOCK) return fail(who, "a leading dimension is below its columns");
+    if (rows && n && (!x || !q || !scale)) return fail(who, "null pointer");
+    return 0;
+}
+unsigned grid_of(int64_t items) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((items + 255) / 256, 256 * 32)); }
+
+}  // namespace
+}  // namespace layers
+}  // namespace smrt
+
+using namespace smrt::layers;
+
+extern "C" int smrt_dense_forward(const smrt_dense* p, void* hip_stream) {
+    const char* who = "smrt_dense_forward";
+    if (int rc = check_dense(p, who)) return rc;
+    if (p->x_scale) return fail(who, "x must be a matrix of dtype: the forward product does not read the 8-bit form");
+    if (p->ldy < p->n || (p->residual && p->ldr < p->n)) return fail(who, "a leading dimension is below its columns");
+    if (p->a && (p->a_scale ? p->lda < pad(p->n, PACK_BLOCK) || p->ld_a_scale < (p->n + PACK_BLOCK - 1) / PACK_BLOCK : p->lda < p->n))
+        return fail(who, "a leading dimension is below its columns");
+    if (p->rows == 0 || p->n == 0) return 0;
+    if (!p->y) return fail(who, "null pointer");
+    const int64_t es = elem_size(p->dtype), y_bytes = span(p->rows, p->ldy, p->n) * es;
+    if (overlap(p->y, y_bytes, p->x, span(p->rows, p->ldx, p->k) * es) ||
+        overlap(p->y, y_bytes, p->w, ((p->groups - 1) * p->w_stride + span(p->k, p->ldw, p->n)) * es) ||
+        (p->residual && (p->residual != p->y || p->ldr != p->ldy) && overlap(p->y, y_bytes, p->residual, span(p->rows, p->ldr, p->n) * es)))
+        return fail(who, "y overlaps an input (it may only be the residual itself)");
+    GemmArgs g = {};
+    g.A = p->x; g.lda = p->ldx; g.B = p->w; g.ldb = p->ldw; g.strideB = p->w_stride; g.C = p->y; g.ldc = p->ldy;
+    g.bias = p->bias; g.stride_bias = p->bias_stride; g.residual = p->residual; g.ldr = p->ldr;
+    if (p->a && p->a_scale) { g.q_out = (int8_t*)p->a; g.ldq = p->lda; g.q_scale = p->a_scale; g.ldq_scale = p->ld_a_scale; }
+    else if (p->a) { g.act_out = p->a; g.ld_act = p->lda; }
+    g.ends = p->ends; g.groups = p->groups; g.keep_rest = p->keep_rest; g.rows = (int32_t)p->rows;
+    g.M = (int32_t)p->rows; g.N = (int32_t)p->n; g.K = (int32_t)p->k; g.splits = 1; g.act = p->activation;
+    return launched(who, gemm(p->dtype, LAYOUT_FORWARD, g, (hipStream_t)hip_stream));
+}
+
+extern "C" int64_t smrt_dense_backward_workspace(const smrt_dense* p) {
+    if (check_dense(p, "smrt_dense_backward_workspace")) return -1;
+    return plan_backward(p).total;
+}
+
+extern "C" int smrt_dense_backward(const smrt_dense* p, void* workspace, int64_t workspace_bytes, void* hip_stream) {
+    const char* who = "smrt_dense_backward";
+    if (int rc = check_dense(p, who)) return rc;
+    const hipStream_t stream = (hipStream_t)hip_stream;
+    const bool packed_a = p->a_scale != nullptr;
+    if (p->ldg < p->n || (p->dx && p->lddx < p->k) || (p->dw && p->lddw < p->n)) return fail(who, "a leading dimension is below its columns");
+    if (p->x_scale && (p->ldx < pad(p->k, PACK_BLOCK) || p->ld_x_scale < (p->k + PACK_BLOCK - 1) / PACK_BLOCK))
+        return fail(who, "a leading dimension is below its columns");
+    if (p->dw && p->groups > 1 && p->dw_stride < span(p->k, p->lddw, p->n)) return fail(who, "the groups' weight gradients overlap");
+    const BackwardPlan b = plan_backward(p);
+    if (b.need_dz && p->rows && p->n) {
+        if (!p->a) return fail(who, "the activation's value is needed");
+        if (packed_a ? p->lda < pad(p->n, PACK_BLOCK) || p->ld_a_scale < (p->n + PACK_BLOCK - 1) / PACK_BLOCK : p->lda < p->n)
+            return fail(who, "a leading dimension is below its columns");
+    }
+    if (p->rows && p->n && !p->grad) return fail(who, "null pointer");
+    if (b.total > workspace_bytes || (b.total && !workspace)) return fail(who, "the workspace is smaller than smrt_dense_backward_workspace says");
+    char* const ws = (char*)workspace;
+    const void* dz = p->grad;
+    int64_t ld_dz = p->ldg;
+    float* const part = b.part_bytes ? (float*)(ws + b.part_off) : nullptr;
+    if (p->n && (b.need_dz || b.need_sum)) {
+        DzArgs d = {};
+        d.grad = p->grad; d.ldg = p->ldg; d.a = p->a; d.lda = p->lda;
+        d.a_scale = b.need_dz ? p->a_scale : nullptr; d.ld_a_scale = p->ld_a_scale;
+        if (b.need_dz) { d.dz = ws; d.ld_dz = b.ld_dz; dz = ws; ld_dz = b.ld_dz; }
+        d.part = part; d.db = p->db; d.db_stride = p->bias_stride;
+        d.ends = p->ends; d.groups = p->groups; d.rows = (int32_t)p->rows; d.n = (int32_t)p->n; d.slices = b.dz_slices; d.act = p->activation;
+        d.col_blocks = (int32_t)((p->n + 255) / 256);
+        if (hipError_t e = by_type(p->dtype, [&](auto t) { return launch_dz<decltype(t)>(d, stream); }); e != hipSuccess) return launched(who, e);
+    }
+    GemmArgs g = {};
+    g.ends = p->ends; g.groups = p->groups; g.keep_rest = p->keep_rest; g.rows = (int32_t)p->rows; g.splits = 1;
+    if (p->dx && p->rows && p->k) {
+        g.A = dz; g.lda = ld_dz; g.B = p->w; g.ldb = p->ldw; g.strideB = p->w_stride; g.C = p->dx; g.ldc = p->lddx;
+        g.M = (int32_t)p->rows; g.N = (int32_t)p->k; g.K = (int32_t)p->n;
+        if (hipError_t e = gemm(p->dtype, LAYOUT_DX, g, stream); e != hipSuccess) return launched(who, e);
+    }
+    const bool dw = p->dw && p->k && p->n;
+    if (dw) {
+        g.A = p->x; g.lda = p->ldx; g.A_scale = p->x_scale; g.lds_scale = p->ld_x_scale; g.B = dz; g.ldb = ld_dz; g.strideB = 0;
+        g.C = p->dw; g.ldc = p->lddw; g.strideC = p->dw_stride; g.slab = b.slab_bytes ? (float*)(ws + b.slab_off) : nullptr;
+        g.M = (int32_t)p->k; g.N = (int32_t)p->n; g.K = (int32_t)p->rows; g.splits = b.splits;
+        if (hipError_t e = gemm(p->dtype, LAYOUT_DW, g, stream); e != hipSuccess) return launched(who, e);
+    }
+    if ((dw && b.slab_bytes) || part) {
+        JoinPart jw = {}, jb = {};
+        if (dw && b.slab_bytes) jw = join_part((const float*)(ws + b.slab_off), b.splits, p->groups * p->k * p->n, p->groups * p->k, p->n, p->dw, p->lddw, p->k, p->dw_stride, false, 1);
+        if (part && p->n) jb = join_part(part, b.dz_slices, p->groups * p->n, p->groups, p->n, p->db, 0, 1, p->bias_stride, false, 32);
+        if (jw.blocks + jb.blocks) {
+            const hipError_t e = by_type(p->dtype, [&](auto t) {
+                hipLaunchKernelGGL((join_kernel<decltype(t), 1, 32>), dim3(jw.blocks + jb.blocks), dim3(256), 0, stream, jw, jb);
+                return hipGetLastError();
+            });
+            if (e != hipSuccess) return launched(who, e);
+        }
+    }
+    return 0;
+}
+
+extern "C" int smrt_layer_norm_forward(const smrt_layer_norm* p, void* hip_stream) {
+    const char* who = "smrt_layer_norm_forward";
+    if (int rc = check_norm(p, who)) return rc;
+    if (p->x_scale) return fail(who, "x must be a matrix of dtype: the forward pass does not read the 8-bit form");
+    if (p->ldy < p->n) return fail(who, "a leading dimension is below its columns");
+    if (p->rows == 0) return 0;
+    if (!p->y) return fail(who, "null pointer");
+    if (!(p->eps >= 0.0f)) return fail(who, "eps must be >= 0");
+    const int64_t es = elem_size(p->dtype);
+    if ((p->x != p->y || p->ldx != p->ldy) && overlap(p->y, span(p->rows, p->ldy, p->n) * es, p->x, span(p->rows, p->ldx, p->n) * es))
+        return fail(who, "y overlaps x (it may only be x itself)");
+    const NormArgs a = norm_args(p);
+    return launched(who, by_type(p->dtype, [&](auto t) {
+        return by_width(p->n, [&](auto tpr, auto ch) {
+            constexpr int TPR = decltype(tpr)::value, THREADS = TPR > 256 ? TPR : 256;
+            hipLaunchKernelGGL((norm_forward_kernel<decltype(t), TPR, decltype(ch)::value>), dim3(norm_blocks(p->rows, THREADS / TPR, 4096)), dim3(THREADS), 0,
+                               (hipStream_t)hip_stream, a);
+            return hipGetLastError();
+        });
+    }));
+}
+
+extern "C" int64_t smrt_layer_norm_backward_workspace(const smrt_layer_norm* p) {
+    if (check_norm(p, "smrt_layer_norm_backward_workspace")) return -1;
+    const int blocks = norm_backward_blocks(p->rows, p->n);
+    return blocks > 1 && (p->dw || p->db) ? (int64_t)blocks * 2 * p->n * 4 : 0;
+}
+
+extern "C" int smrt_layer_norm_backward(const smrt_layer_norm* p, void* workspace, int64_t workspace_bytes, void* hip_stream) {
+    const char* who = "smrt_layer_norm_backward";
+    if (int rc = check_norm(p, who)) return rc;
+    const hipStream_t stream = (hipStream_t)hip_stream;
+    if (p->ldg < p->n || (p->dx && p->lddx < p->n)) return fail(who, "a leading dimension is below its columns");
+    if (p->x_scale && (p->ldx < pad(p->n, PACK_BLOCK) || p->ld_x_scale < (p->n + PACK_BLOCK - 1) / PACK_BLOCK))
+        return fail(who, "a leading dimension is below its columns");
+    if (p->rows && !p->grad) return fail(who, "null pointer");
+    const int64_t need = smrt_layer_norm_backward_workspace(p);
+    if (need > workspace_bytes || (need && !workspace)) return fail(who, "the workspace is smaller than smrt_layer_norm_backward_workspace says");
+    NormArgs a = norm_args(p);
+    const int blocks = norm_backward_blocks(p->rows, p->n);
+    a.part = need ? (float*)workspace : nullptr;
+    hipError_t e = by_type(p->dtype, [&](auto t) {
+        return by_width(p->n, [&](auto tpr, auto ch) {
+            constexpr int TPR = decltype(tpr)::value, CH = decltype(ch)::value, THREADS = TPR > 256 ? TPR : 256;
+            if (p->x_scale) hipLaunchKernelGGL((norm_backward_kernel<decltype(t), true, TPR, CH>), dim3(blocks), dim3(THREADS), 0, stream, a);
+            else hipLaunchKernelGGL((norm_backward_kernel<decltype(t), false, TPR, CH>), dim3(blocks), dim3(THREADS), 0, stream, a);
+            return hipGetLastError();
+        });
+    });
+    if (e == hipSuccess && a.part) {
+        // slabs of 2 n: the weight's half, then the bias's
+        JoinPart jw = {}, jb = {};
+        const bool f32 = a.w_f32;
+        if (p->dw) jw = join_part(a.part, blocks, 2 * p->n, 1, p->n, p->dw, 0, 1, 0, f32, 32);
+        if (p->db) jb = join_part(a.part + p->n, blocks, 2 * p->n, 1, p->n, p->db, 0, 1, 0, f32, 32);
+        e = by_type(p->dtype, [&](auto t) {
+            hipLaunchKernelGGL((join_kernel<decltype(t), 32, 32>), dim3(jw.blocks + jb.blocks), dim3(256), 0, stream, jw, jb);
+            return hipGetLastError();
+        });
+    }
+    return launched(who, e);
+}
+
+extern "C" int smrt_pack_rows(int32_t dtype, const void* x, int64_t ldx, int64_t rows, int64_t n, int8_t* q, int64_t ldq, uint8_t* scale,
+                              int64_t ld_scale, void* hip_stream) {
+    const char* who = "smrt_pack_rows";
+    if (int rc = check_pack(who, dtype, x, ldx, rows, n, q, ldq, scale, ld_scale)) return rc;
+    if (rows == 0 || n == 0) return 0;
+    const PackArgs a = {x, ldx, q, ldq, scale, ld_scale, rows, (int32_t)n, nullptr};
+    return launched(who, by_type(dtype, [&](auto t) {
+        hipLaunchKernelGGL((pack_kernel<decltype(t)>), dim3(grid_of(rows * (pad(n, PACK_BLOCK) / 8))), dim3(256), 0, (hipStream_t)hip_stream, a);
+        return hipGetLastError();
+    }));
+}
+
+extern "C" int smrt_unpack_rows(int32_t dtype, const int8_t* q, int64_t ldq, const uint8_t* scale, int64_t ld_scale, int64_t rows, int64_t n,
+                                void* x, int64_t ldx, void* hip_stream) {
+    const char* who = "smrt_unpack_rows";
+    if (int rc = check_pack(who, dtype, x, ldx, rows, n, q, ldq, scale, ld_scale)) return rc;
+    if (rows == 0 || n == 0) return 0;
+    const PackArgs a = {nullptr, ldx, (int8_t*)q, ldq, (uint8_t*)scale, ld_scale, rows, (int32_t)n, x};
+    return launched(who, by_type(dtype, [&](auto t) {
+        hipLaunchKernelGGL((unpack_kernel<decltype(t)>), dim3(grid_of(rows * ((n + 7) / 8))), dim3(256), 0, (hipStream_t)hip_stream, a);
+        return hipGetLastError();
+    }));
+}

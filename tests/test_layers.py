@@ -1,0 +1,156 @@
+"""Layer operators (smrt_amd.autoencode.layers) without a GPU: what they refuse, and the C entries' own argument checks."""
+import ctypes as C
+
+import pytest
+import torch
+
+from smrt_amd import _hip
+from smrt_amd.autoencode import (PackedRows, dense, dense_backward, dense_grouped, dense_grouped_backward, layer_norm,
+                                 layer_norm_backward, pack_rows, unpack_rows)
+
+
+def t(*shape, dtype=torch.float32):
+    return torch.zeros(shape, dtype=dtype)
+
+
+def packed(rows, cols, dtype=torch.float32):
+    b = -(-cols // 32)
+    return PackedRows(t(rows, 32 * b, dtype=torch.int8), t(rows, b, dtype=torch.uint8), cols, dtype)
+
+
+REFUSED = [
+    ("x is no tensor", TypeError, lambda: dense([[1.0]], t(1, 1))),
+    ("x of another type", ValueError, lambda: dense(t(2, 3, dtype=torch.float64), t(3, 4, dtype=torch.float64))),
+    ("x 1-d", ValueError, lambda: dense(t(3), t(3, 4))),
+    ("x 3-d", ValueError, lambda: dense(t(2, 2, 3), t(3, 4))),
+    ("weight of another type", ValueError, lambda: dense(t(2, 3), t(3, 4, dtype=torch.bfloat16))),
+    ("weight of another depth", ValueError, lambda: dense(t(2, 3), t(4, 4))),
+    ("weight transposed", ValueError, lambda: dense(t(2, 3), t(4, 3).t())),
+    ("rows that overlap", ValueError, lambda: dense(t(1, 3).expand(2, 3), t(3, 4))),
+    ("bias shape", ValueError, lambda: dense(t(2, 3), t(3, 4), t(3))),
+    ("bias 2-d", ValueError, lambda: dense(t(2, 3), t(3, 4), t(1, 4))),
+    ("residual shape", ValueError, lambda: dense(t(2, 3), t(3, 4), residual=t(1, 4))),
+    ("residual type", ValueError, lambda: dense(t(2, 3), t(3, 4), residual=t(2, 4, dtype=torch.float16))),
+    ("out shape", ValueError, lambda: dense(t(2, 3), t(3, 4), out=t(2, 5))),
+    ("activation", ValueError, lambda: dense(t(2, 3), t(3, 4), activation="gelu")),
+    ("activation no text", ValueError, lambda: dense(t(2, 3), t(3, 4), activation=[])),
+    ("save", ValueError, lambda: dense(t(2, 3), t(3, 4), save="all")),
+    ("requires grad", ValueError, lambda: dense(t(2, 3).requires_grad_(), t(3, 4))),
+    ("packed x in the forward pass", TypeError, lambda: dense(packed(2, 3), t(3, 4))),
+    ("backward without saved", ValueError, lambda: dense_backward(t(2, 4), t(2, 3), t(3, 4), activation="relu")),
+    ("backward grad shape", ValueError, lambda: dense_backward(t(2, 5), t(2, 3), t(3, 4))),
+    ("backward x rows", ValueError, lambda: dense_backward(t(2, 4), t(3, 3), t(3, 4))),
+    ("backward packed of another type", ValueError, lambda: dense_backward(t(2, 4), packed(2, 3, torch.float16), t(3, 4))),
+    ("backward packed of another shape", ValueError, lambda: dense_backward(t(2, 4), packed(2, 4), t(3, 4))),
+    ("ends missing", TypeError, lambda: dense_grouped(t(2, 3), None, t(1, 3, 4))),
+    ("ends int32", ValueError, lambda: dense_grouped(t(2, 3), t(1, dtype=torch.int32), t(1, 3, 4))),
+    ("ends length", ValueError, lambda: dense_grouped(t(2, 3), t(2, dtype=torch.int64), t(1, 3, 4))),
+    ("no groups", ValueError, lambda: dense_grouped(t(2, 3), t(0, dtype=torch.int64), t(0, 3, 4))),
+    ("grouped weight 2-d", ValueError, lambda: dense_grouped(t(2, 3), t(1, dtype=torch.int64), t(3, 4))),
+    ("grouped weights that overlap", ValueError, lambda: dense_grouped(t(2, 3), t(2, dtype=torch.int64), t(1, 3, 4).expand(2, 3, 4))),
+    ("grouped bias 1-d", ValueError, lambda: dense_grouped(t(2, 3), t(2, dtype=torch.int64), t(2, 3, 4), t(4))),
+    ("grouped backward ends", ValueError, lambda: dense_grouped_backward(t(2, 4), t(2, 3), t(3, dtype=torch.int64), t(2, 3, 4))),
+    ("norm no columns", ValueError, lambda: layer_norm(t(2, 0))),
+    ("norm too wide", ValueError, lambda: layer_norm(t(1, 32769))),
+    ("norm eps", ValueError, lambda: layer_norm(t(2, 3), eps=-1.0)),
+    ("norm eps nan", ValueError, lambda: layer_norm(t(2, 3), eps=float("nan"))),
+    ("norm bias alone", ValueError, lambda: layer_norm(t(2, 3), None, t(3))),
+    ("norm weight type", ValueError, lambda: layer_norm(t(2, 3), t(3, dtype=torch.bfloat16))),
+    ("norm bias type", ValueError, lambda: layer_norm(t(2, 3, dtype=torch.bfloat16), t(3), t(3, dtype=torch.bfloat16))),
+    ("norm weight length", ValueError, lambda: layer_norm(t(2, 3), t(4))),
+    ("norm backward mean", ValueError, lambda: layer_norm_backward(t(2, 3), t(2, 3), t(3), t(2))),
+    ("norm backward rstd type", ValueError, lambda: layer_norm_backward(t(2, 3), t(2, 3), t(2), t(2, dtype=torch.float16))),
+    ("pack int", ValueError, lambda: pack_rows(t(2, 3, dtype=torch.int8))),
+    ("unpack tensor", TypeError, lambda: unpack_rows(t(2, 3))),
+    ("packed q shape", ValueError, lambda: PackedRows(t(2, 3, dtype=torch.int8), t(2, 1, dtype=torch.uint8), 3, torch.float32)),
+    ("packed scale shape", ValueError, lambda: PackedRows(t(2, 64, dtype=torch.int8), t(2, 1, dtype=torch.uint8), 33, torch.float32)),
+    ("packed dtype", ValueError, lambda: PackedRows(t(2, 32, dtype=torch.int8), t(2, 1, dtype=torch.uint8), 3, torch.float64)),
+]
+
+
+@pytest.mark.parametrize("what,error,call", REFUSED, ids=[r[0] for r in REFUSED])
+def test_refused(what, error, call):
+    with pytest.raises(error):
+        call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: dense(t(2, 3), t(3, 4)), lambda: dense_backward(t(2, 4), t(2, 3), t(3, 4)),
+    lambda: dense_grouped(t(2, 3), t(1, dtype=torch.int64), t(1, 3, 4)),
+    lambda: layer_norm(t(2, 3)), lambda: layer_norm_backward(t(2, 3), t(2, 3), t(2), t(2)),
+    lambda: pack_rows(t(2, 3)), lambda: unpack_rows(packed(2, 3))])
+def test_no_cpu_fallback(call):
+    with pytest.raises(_hip.HipLibraryError):
+        call()
+
+
+def _dense_args(**kw):
+    """A sound call on made-up addresses that is refused for what `kw` changes; nothing is launched before the checks."""
+    base = dict(dtype=0, activation=3, rows=4, k=8, n=16, groups=1, x=0x10000, ldx=8, w=0x20000, ldw=16, w_stride=0, bias_stride=16,
+                y=0x30000, ldy=16, a=0x40000, lda=16, grad=0x50000, ldg=16, dx=0x60000, lddx=8, dw=0x70000, lddw=16, dw_stride=128, db=0x80000)
+    return _hip.Dense(**{**base, **kw})
+
+
+FORWARD_BAD = [dict(dtype=3), dict(dtype=-1), dict(activation=5), dict(rows=-1), dict(rows=1 << 31), dict(k=1 << 31), dict(groups=0),
+               dict(groups=2), dict(groups=1 << 16, ends=0x1000), dict(ldx=7), dict(ldw=15), dict(ldy=15), dict(lda=15), dict(x=0), dict(w=0), dict(y=0),
+               dict(x_scale=0x90000), dict(residual=0x100000, ldr=15), dict(groups=2, ends=0x1000, w_stride=64), dict(w_stride=-1),
+               dict(groups=2, ends=0x1000, w_stride=128, bias=0x1000, bias_stride=15),
+               dict(a_scale=0x90000, lda=16), dict(a_scale=0x90000, lda=32, ld_a_scale=0),
+               dict(y=0x10000), dict(y=0x20010), dict(residual=0x30010, ldr=16), dict(residual=0x30000, ldr=20)]
+
+
+@pytest.mark.parametrize("kw", FORWARD_BAD, ids=str)
+def test_dense_forward_entry_refuses(kw):
+    args = _dense_args(**kw)
+    assert _hip.load().smrt_dense_forward(C.byref(args), None) == -1
+    assert b"smrt_dense_forward" in _hip.load().smrt_last_error()
+
+
+BACKWARD_BAD = [dict(dtype=3), dict(groups=0), dict(ldg=15), dict(lddx=7), dict(lddw=15), dict(grad=0), dict(a=0), dict(lda=15), dict(x=0),
+                dict(x_scale=0x90000, ldx=8), dict(x_scale=0x90000, ldx=32, ld_x_scale=0), dict(a_scale=0x90000, lda=16),
+                dict(groups=2, ends=0x1000, w_stride=128, dw_stride=100)]
+
+
+@pytest.mark.parametrize("kw", BACKWARD_BAD, ids=str)
+def test_dense_backward_entry_refuses(kw):
+    args = _dense_args(**kw)
+    assert _hip.load().smrt_dense_backward(C.byref(args), 0xa0000, 1 << 20, None) == -1
+
+
+def test_entries_refuse_null_and_small_workspaces():
+    lib = _hip.load()
+    assert lib.smrt_dense_forward(None, None) == -1
+    assert lib.smrt_dense_backward(None, None, 0, None) == -1
+    assert lib.smrt_dense_backward_workspace(None) == -1
+    assert lib.smrt_layer_norm_forward(None, None) == -1
+    assert lib.smrt_layer_norm_backward(None, None, 0, None) == -1
+    assert lib.smrt_layer_norm_backward_workspace(None) == -1
+    args = _dense_args()
+    need = lib.smrt_dense_backward_workspace(C.byref(args))
+    assert need > 0
+    assert lib.smrt_dense_backward(C.byref(args), 0xa0000, need - 1, None) == -1
+    assert lib.smrt_dense_backward(C.byref(args), None, need, None) == -1
+    norm = dict(dtype=1, rows=4000, n=64, eps=1e-5, x=0x10000, ldx=64, y=0x200000, ldy=64, mean=0x900000, rstd=0xa00000, grad=0xb00000, ldg=64,
+                dx=0xc00000, lddx=64, dw=0xd00000, db=0xe00000)
+    args = _hip.LayerNorm(**norm)
+    need = lib.smrt_layer_norm_backward_workspace(C.byref(args))
+    assert need > 0
+    assert lib.smrt_layer_norm_backward(C.byref(args), 0x10000, need - 1, None) == -1
+    for kw in (dict(dtype=9), dict(n=0), dict(n=32769), dict(rows=-1), dict(ldx=63), dict(ldy=63), dict(x=0), dict(y=0), dict(mean=0), dict(eps=-1.0),
+               dict(x_scale=0x1000), dict(y=0x10080)):
+        args = _hip.LayerNorm(**{**norm, **kw})
+        assert lib.smrt_layer_norm_forward(C.byref(args), None) == -1, kw
+    for kw in (dict(ldg=63), dict(lddx=63), dict(grad=0), dict(x_scale=0x1000, ld_x_scale=1)):
+        args = _hip.LayerNorm(**{**norm, **kw})
+        assert lib.smrt_layer_norm_backward(C.byref(args), 0x10000, 1 << 30, None) == -1, kw
+
+
+def test_pack_entries_refuse():
+    lib = _hip.load()
+    good = [0, 0x1000, 40, 4, 40, 0x2000, 64, 0x3000, 2]
+    for i, v in ((0, 3), (1, 0), (2, 39), (3, -1), (4, -1), (5, 0), (6, 63), (7, 0), (8, 1)):
+        bad = list(good)
+        bad[i] = v
+        assert lib.smrt_pack_rows(*bad, None) == -1, (i, v)
+        dt, x, ldx, rows, n, q, ldq, s, lds = bad
+        assert lib.smrt_unpack_rows(dt, q, ldq, s, lds, rows, n, x, ldx, None) == -1, (i, v)
