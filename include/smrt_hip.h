@@ -270,7 +270,7 @@ int  smrt_smote_rows_f64(const double* X_dev, int64_t n_x, int64_t ldx, int64_t 
  * the handles above run inside one net, for nets that are put together from layers.
  *
  * Types: SMRT_F32, SMRT_BF16, SMRT_F16; sums are fp32.  Matrices are row-major DEVICE memory, elements of a row next to each
- * other, a leading dimension (in elements) for each; rows may start at any element.  Work is queued on hip_stream, nothing is
+ * other, a leading dimension (in elements, at most 2^21 for what a product reads) for each; rows may start at any element.  Work is queued on hip_stream, nothing is
  * allocated, nothing waits: the calls can be captured into a graph.  Workspaces are the caller's, not shared by calls that may
  * run at the same time.  Sizes may be 0.  Returns 0, or -1 (bad argument, nothing was done) or -2 (launch failed).
  *

@@ -26,11 +26,17 @@ from .. import _hip
 __all__ = ["dense", "dense_backward", "dense_grouped", "dense_grouped_backward", "layer_norm", "layer_norm_backward",
            "pack_rows", "unpack_rows", "PackedRows"]
 
+_Tensor = torch.Tensor
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _BLOCK = 32                                      # columns that share a scale byte
 
 
-def _tensor(t, name, dim, dtype=None, device=None):
+# A small layer is over in a few microseconds, so the checks have a short way for the usual argument -- a plain tensor of the
+# right type, device and layout -- and words only for the others.
+def _tensor(t, name, dim, dtype, dev):
+    """Checks any tensor argument; ``dtype`` None: one of the three types, ``dev`` None: any device."""
+    if type(t) is _Tensor and t.dtype is dtype and t.get_device() == dev and not t.requires_grad and t.is_contiguous() and t.dim() == dim:
+        return t
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a torch tensor, got %s" % (name, type(t).__name__))
     if t.dim() != dim:
@@ -40,16 +46,16 @@ def _tensor(t, name, dim, dtype=None, device=None):
             raise ValueError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
     elif t.dtype != dtype:
         raise ValueError("%s must be %s, got %s" % (name, dtype, t.dtype))
-    if device is not None and t.device != device:
-        raise ValueError("%s is on %s, expected %s" % (name, t.device, device))
+    if dev is not None and t.get_device() != dev:
+        raise ValueError("%s is on %s, expected %s" % (name, t.device, "the CPU" if dev < 0 else "cuda:%d" % dev))
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError("%s requires grad, and the layer calls take no part in autograd: detach it, or call under torch.no_grad()" % name)
-    if dim and t.shape[-1] > 1 and t.stride(-1) != 1 and t.numel():
+    if t.shape[-1] > 1 and t.stride(-1) != 1 and t.numel():
         raise ValueError("the elements of a row of %s must lie next to each other (strides %r)" % (name, t.stride()))
     return t
 
 
-def _ld(t, name="matrix"):
+def _ld(t, name):
     """Leading dimension of a matrix (of the last two dimensions)."""
     rows, cols = t.shape[-2:]
     if rows <= 1 or cols == 0:
@@ -60,26 +66,49 @@ def _ld(t, name="matrix"):
     return ld
 
 
+def _matrix(t, name, dtype, dev):
+    """Checks a matrix argument: ``(rows, cols, leading dimension)``."""
+    if type(t) is _Tensor and (t.dtype is dtype or dtype is None and t.dtype in _DTYPES) and t.get_device() == dev and not t.requires_grad:
+        stride = t.stride()
+        if len(stride) == 2 and stride[1] == 1:
+            rows, cols = t.shape
+            if stride[0] >= cols > 0:
+                return rows, cols, stride[0]
+    _tensor(t, name, 2, dtype, dev)
+    return t.shape[0], t.shape[1], _ld(t, name)
+
+
 def _shape(t, name, shape):
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError("%s must have shape %r, got %r" % (name, tuple(shape), tuple(t.shape)))
+    if t.shape != shape:
+        raise ValueError("%s must have shape %r, got %r" % (name, shape, tuple(t.shape)))
 
 
-def _on_gpu(t):
-    if not t.is_cuda:
-        raise _hip.HipLibraryError("the layer calls run on an MI355X; there is no CPU fallback (got a tensor on %s)" % t.device)
+def _device_of(t, name):
+    """Ordinal of a tensor's GPU, -1 for the CPU."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch tensor, got %s" % (name, type(t).__name__))
+    return t.get_device()
 
 
-def _call(device, fn, what, *args):
+def _on_gpu(dev):
+    if dev < 0:
+        raise _hip.HipLibraryError("the layer calls run on an MI355X; there is no CPU fallback (got tensors on the CPU)")
+
+
+# what torch.cuda.current_stream(dev).cuda_stream and torch.cuda.current_device() come to, without their objects
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _call(dev, fn, *args):
     """``fn(*args, stream)`` on the device's current stream, with that device current."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, stream)
+    if _current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, stream)
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
     if rc:
-        raise _hip.HipLibraryError("%s failed (%d): %s" % (what, rc, _hip.load().smrt_last_error().decode()))
+        raise _hip.HipLibraryError("%s failed (%d): %s" % (fn.__name__, rc, _hip.load().smrt_last_error().decode()))
 
 
 def _activation(name):
@@ -104,11 +133,13 @@ class PackedRows(object):
         cols = int(cols)
         if dtype not in _DTYPES:
             raise ValueError("dtype must be float32, bfloat16 or float16, got %s" % dtype)
-        _tensor(q, "q", 2, torch.int8)
-        _tensor(scale, "scale", 2, torch.uint8, q.device)
+        dev = _device_of(q, "q")
+        _tensor(q, "q", 2, torch.int8, dev)
+        _tensor(scale, "scale", 2, torch.uint8, dev)
         blocks = -(-cols // _BLOCK)
         _shape(q, "q", (q.shape[0], blocks * _BLOCK))
         _shape(scale, "scale", (q.shape[0], blocks))
+        _ld(q, "q"), _ld(scale, "scale")
         self.q, self.scale, self.cols, self.dtype = q, scale, cols, dtype
 
     @property
@@ -134,13 +165,12 @@ def _new_packed(rows, cols, dtype, device):
 
 def pack_rows(x):
     """The 8-bit form of ``x`` ``[rows, cols]`` (``PackedRows``)."""
-    _tensor(x, "x", 2)
-    ld = _ld(x, "x")
-    _on_gpu(x)
-    rows, cols = x.shape
+    dev = _device_of(x, "x")
+    rows, cols, ld = _matrix(x, "x", None, dev)
+    _on_gpu(dev)
     p = _new_packed(rows, cols, x.dtype, x.device)
-    _call(x.device, _hip.load().smrt_pack_rows, "smrt_pack_rows", _DTYPES[x.dtype], x.data_ptr(), ld, rows, cols, p.q.data_ptr(), p.q.shape[1],
-          p.scale.data_ptr(), p.scale.shape[1])
+    _call(dev, _hip.load().smrt_pack_rows, _DTYPES[x.dtype], x.data_ptr(), ld, rows, cols, p.q.data_ptr(), p.q.shape[1], p.scale.data_ptr(),
+          p.scale.shape[1])
     return p
 
 
@@ -148,114 +178,124 @@ def unpack_rows(packed):
     """The values that ``packed`` stands for, a tensor ``[rows, cols]`` of ``packed.dtype``."""
     if not isinstance(packed, PackedRows):
         raise TypeError("packed must be PackedRows, got %s" % type(packed).__name__)
-    _on_gpu(packed.q)
-    rows, cols = packed.shape
-    out = torch.empty((rows, cols), dtype=packed.dtype, device=packed.device)
-    _call(packed.device, _hip.load().smrt_unpack_rows, "smrt_unpack_rows", _DTYPES[packed.dtype], packed.q.data_ptr(), _ld(packed.q, "q"),
-          packed.scale.data_ptr(), _ld(packed.scale, "scale"), rows, cols, out.data_ptr(), max(cols, 1))
+    q, scale, cols = packed.q, packed.scale, packed.cols
+    dev, rows = q.get_device(), q.shape[0]
+    _on_gpu(dev)
+    out = torch.empty((rows, cols), dtype=packed.dtype, device=q.device)
+    _call(dev, _hip.load().smrt_unpack_rows, _DTYPES[packed.dtype], q.data_ptr(), _ld(q, "q"), scale.data_ptr(), _ld(scale, "scale"), rows, cols,
+          out.data_ptr(), cols or 1)
     return out
 
 
-def _kept(t, name, shape, dtype, device):
+def _kept(t, name, rows, cols, dtype, dev):
     """A tensor or PackedRows of an earlier pass: ``(pointer, ld, scale pointer, scale ld)``."""
     if isinstance(t, PackedRows):
-        if t.dtype != dtype or t.shape != tuple(shape) or t.device != device:
-            raise ValueError("%s must be a %s matrix of shape %r on %s, got %r" % (name, dtype, tuple(shape), device, t))
-        return t.q.data_ptr(), _ld(t.q, name), t.scale.data_ptr(), _ld(t.scale, name)
-    _tensor(t, name, 2, dtype, device)
-    _shape(t, name, shape)
-    return t.data_ptr(), _ld(t, name), None, 0
+        q, scale = t.q, t.scale
+        if t.dtype != dtype or q.shape[0] != rows or t.cols != cols or q.get_device() != dev:
+            raise ValueError("%s must be a %s matrix of shape %r on the others' device, got %r" % (name, dtype, (rows, cols), t))
+        return q.data_ptr(), _ld(q, name), scale.data_ptr(), _ld(scale, name)
+    r, c, ld = _matrix(t, name, dtype, dev)
+    if r != rows or c != cols:
+        _shape(t, name, (rows, cols))
+    return t.data_ptr(), ld, None, 0
 
 
 # ------------------------------------------------------------------------------------------------ dense
-def _weights(weight, bias, x_dtype, device, k, ends):
-    """Checks of a weight ``[k, n]`` or ``[groups, k, n]``, its bias and the groups' ends: ``(n, groups, ldw, w_stride, bias_stride)``."""
-    grouped = ends is not None
-    _tensor(weight, "weight", 3 if grouped else 2, x_dtype, device)
-    if weight.shape[-2] != k:
-        raise ValueError("x has %d columns, weight has shape %r" % (k, tuple(weight.shape)))
-    n, groups = weight.shape[-1], weight.shape[0] if grouped else 1
-    ldw = _ld(weight, "weight")
-    w_stride = weight.stride(0) if grouped and groups > 1 else 0
-    if grouped:
-        _tensor(ends, "ends", 1, torch.int64, device)
-        _shape(ends, "ends", (groups,))
-        if not 1 <= groups <= 65535:
-            raise ValueError("between 1 and 65535 groups are supported, got %d" % groups)
-        if groups > 1 and w_stride < (k - 1) * ldw + n:
-            raise ValueError("the weights of the groups overlap (strides %r)" % (weight.stride(),))
-    bias_stride = n
-    if bias is not None:
-        _tensor(bias, "bias", 2 if grouped else 1, x_dtype, device)
-        _shape(bias, "bias", (groups, n) if grouped else (n,))
-        bias_stride = _ld(bias, "bias") if grouped else n
-    return n, groups, ldw, w_stride, bias_stride
+def _weights(weight, bias, dtype, dev, ends):
+    """Checks of a weight ``[k, n]`` or ``[groups, k, n]``, its bias and the groups' ends: ``(k, n, groups, ldw, w_stride, bias pointer, bias_stride)``."""
+    if ends is None:
+        k, n, ldw = _matrix(weight, "weight", dtype, dev)
+        if bias is None:
+            return k, n, 1, ldw, 0, None, n
+        _tensor(bias, "bias", 1, dtype, dev)
+        if bias.shape[0] != n:
+            _shape(bias, "bias", (n,))
+        return k, n, 1, ldw, 0, bias.data_ptr(), n
+    _tensor(weight, "weight", 3, dtype, dev)
+    groups, k, n = weight.shape
+    _tensor(ends, "ends", 1, torch.int64, dev)
+    _shape(ends, "ends", (groups,))
+    if not 1 <= groups <= 65535:
+        raise ValueError("between 1 and 65535 groups are supported, got %d" % groups)
+    ldw, w_stride = _ld(weight, "weight"), weight.stride(0) if groups > 1 else 0
+    if groups > 1 and w_stride < (k - 1) * ldw + n:
+        raise ValueError("the weights of the groups overlap (strides %r)" % (weight.stride(),))
+    if bias is None:
+        return k, n, groups, ldw, w_stride, None, n
+    b_rows, b_cols, bias_stride = _matrix(bias, "bias", dtype, dev)
+    if b_rows != groups or b_cols != n:
+        _shape(bias, "bias", (groups, n))
+    return k, n, groups, ldw, w_stride, bias.data_ptr(), bias_stride
 
 
 def _dense(x, ends, weight, bias, residual, activation, save, out):
     act = _activation(activation)
-    if save not in (None, "activation", "packed"):
+    if save is not None and save not in ("activation", "packed"):
         raise ValueError("save must be None, 'activation' or 'packed', got %r" % (save,))
-    _tensor(x, "x", 2)
-    dtype, device = x.dtype, x.device
-    rows, k = x.shape
-    n, groups, ldw, w_stride, bias_stride = _weights(weight, bias, dtype, device, k, ends)
-    ldx = _ld(x, "x")
+    dev = _device_of(x, "x")
+    rows, xk, ldx = _matrix(x, "x", None, dev)
+    dtype = x.dtype
+    k, n, groups, ldw, w_stride, b_ptr, bias_stride = _weights(weight, bias, dtype, dev, ends)
+    if xk != k:
+        raise ValueError("x has %d columns, weight has shape %r" % (xk, tuple(weight.shape)))
     r_ptr, ldr = None, 0
     if residual is not None:
-        _tensor(residual, "residual", 2, dtype, device)
-        _shape(residual, "residual", (rows, n))
-        r_ptr, ldr = residual.data_ptr(), _ld(residual, "residual")
-    if out is not None:
-        _tensor(out, "out", 2, dtype, device)
-        _shape(out, "out", (rows, n))
-    _on_gpu(x)
-    y = torch.empty((rows, n), dtype=dtype, device=device) if out is None else out
+        r_rows, r_cols, ldr = _matrix(residual, "residual", dtype, dev)
+        if r_rows != rows or r_cols != n:
+            _shape(residual, "residual", (rows, n))
+        r_ptr = residual.data_ptr()
+    if out is None:
+        _on_gpu(dev)
+        y, ldy = torch.empty((rows, n), dtype=dtype, device=x.device), n or 1
+    else:
+        y_rows, y_cols, ldy = _matrix(out, "out", dtype, dev)
+        if y_rows != rows or y_cols != n:
+            _shape(out, "out", (rows, n))
+        _on_gpu(dev)
+        y = out
     saved, a_ptr, lda, s_ptr, lds = None, None, 0, None, 0
     if save is not None and act != 1:                      # the identity's derivative needs nothing
         if save == "packed":
-            saved = _new_packed(rows, n, dtype, device)
+            saved = _new_packed(rows, n, dtype, x.device)
             a_ptr, lda, s_ptr, lds = saved.q.data_ptr(), saved.q.shape[1], saved.scale.data_ptr(), saved.scale.shape[1]
         elif residual is None:
             saved = y
         else:
-            saved = torch.empty((rows, n), dtype=dtype, device=device)
+            saved = torch.empty((rows, n), dtype=dtype, device=x.device)
             a_ptr, lda = saved.data_ptr(), n
     args = _hip.Dense(_DTYPES[dtype], act, rows, k, n, groups, out is not None, None if ends is None else ends.data_ptr(),
-                      x.data_ptr(), ldx, None, 0, weight.data_ptr(), ldw, w_stride, None if bias is None else bias.data_ptr(), bias_stride,
-                      r_ptr, ldr, y.data_ptr(), _ld(y, "out"), a_ptr, lda, s_ptr, lds)
-    _call(device, _hip.load().smrt_dense_forward, "smrt_dense_forward", C.byref(args))
+                      x.data_ptr(), ldx, None, 0, weight.data_ptr(), ldw, w_stride, b_ptr, bias_stride, r_ptr, ldr, y.data_ptr(), ldy,
+                      a_ptr, lda, s_ptr, lds)
+    _call(dev, _hip.load().smrt_dense_forward, C.byref(args))
     return y if save is None else (y, saved)
 
 
 def _dense_backward(grad, x, ends, weight, saved, activation, need_x, need_weight, need_bias):
     act = _activation(activation)
-    _tensor(grad, "grad", 2)
+    dev = _device_of(grad, "grad")
+    rows, gn, ldg = _matrix(grad, "grad", None, dev)
     dtype, device = grad.dtype, grad.device
-    k = weight.shape[-2] if isinstance(weight, torch.Tensor) and weight.dim() > 1 else 0
-    n, groups, ldw, w_stride, _ = _weights(weight, None, dtype, device, k, ends)
-    rows = grad.shape[0]
-    _shape(grad, "grad", (rows, n))
-    x_ptr, ldx, xs_ptr, ld_xs = _kept(x, "x", (rows, k), dtype, device)
+    k, n, groups, ldw, w_stride, _, _ = _weights(weight, None, dtype, dev, ends)
+    if gn != n:
+        raise ValueError("grad has %d columns, weight has shape %r" % (gn, tuple(weight.shape)))
+    x_ptr, ldx, xs_ptr, ld_xs = _kept(x, "x", rows, k, dtype, dev)
     a_ptr, lda, as_ptr, ld_as = None, 0, None, 0
     if act != 1:
         if saved is None:
             raise ValueError("the gradient of %r needs what the forward pass saved" % activation)
-        a_ptr, lda, as_ptr, ld_as = _kept(saved, "saved", (rows, n), dtype, device)
-    ldg = _ld(grad, "grad")
-    _on_gpu(grad)
-    lead = () if ends is None else (groups,)
+        a_ptr, lda, as_ptr, ld_as = _kept(saved, "saved", rows, n, dtype, dev)
+    _on_gpu(dev)
     dx = torch.empty((rows, k), dtype=dtype, device=device) if need_x else None
-    dw = torch.empty(lead + (k, n), dtype=dtype, device=device) if need_weight else None
-    db = torch.empty(lead + (n,), dtype=dtype, device=device) if need_bias else None
+    dw = torch.empty(weight.shape, dtype=dtype, device=device) if need_weight else None
+    db = torch.empty((n,) if ends is None else (groups, n), dtype=dtype, device=device) if need_bias else None
     args = _hip.Dense(_DTYPES[dtype], act, rows, k, n, groups, 0, None if ends is None else ends.data_ptr(),
                       x_ptr, ldx, xs_ptr, ld_xs, weight.data_ptr(), ldw, w_stride, None, n, None, 0, None, 0, a_ptr, lda, as_ptr, ld_as,
-                      grad.data_ptr(), ldg, dx.data_ptr() if need_x else None, max(k, 1), dw.data_ptr() if need_weight else None, max(n, 1), k * n,
+                      grad.data_ptr(), ldg, dx.data_ptr() if need_x else None, k or 1, dw.data_ptr() if need_weight else None, n or 1, k * n,
                       db.data_ptr() if need_bias else None)
     lib, ref = _hip.load(), C.byref(args)
     size = lib.smrt_dense_backward_workspace(ref)
-    work = torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
-    _call(device, lib.smrt_dense_backward, "smrt_dense_backward", ref, None if work is None else work.data_ptr(), max(size, 0))
+    work = torch.empty((size,), dtype=torch.uint8, device=device) if size > 0 else None
+    _call(dev, lib.smrt_dense_backward, ref, None if work is None else work.data_ptr(), size)
     return dx, dw, db
 
 
@@ -297,70 +337,75 @@ def _ends(ends):
 
 
 # ------------------------------------------------------------------------------------------------ layer norm
-def _norm_weight(weight, bias, dtype, device, n):
+def _norm_weight(weight, bias, dtype, dev, n):
+    """``(weight is float32, weight pointer, bias pointer)``"""
     if weight is None:
         if bias is not None:
             raise ValueError("bias without weight is not supported")
-        return 0
+        return 0, None, None
     if not isinstance(weight, torch.Tensor) or weight.dtype not in (dtype, torch.float32):
         raise ValueError("weight must be a tensor of %s or float32" % dtype)
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None:
-            _tensor(t, name, 1, weight.dtype, device)
-            _shape(t, name, (n,))
-    return int(weight.dtype == torch.float32)
+    _tensor(weight, "weight", 1, weight.dtype, dev)
+    if weight.shape[0] != n:
+        _shape(weight, "weight", (n,))
+    if bias is not None:
+        _tensor(bias, "bias", 1, weight.dtype, dev)
+        if bias.shape[0] != n:
+            _shape(bias, "bias", (n,))
+    return weight.dtype is torch.float32, weight.data_ptr(), None if bias is None else bias.data_ptr()
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
     """``(y, mean, rstd)``: each row of ``x`` ``[rows, n]`` less its mean, over ``sqrt(variance + eps)``, times ``weight`` plus ``bias``
     (``[n]``, of ``x``'s type or float32).  ``mean`` and ``rstd`` are float32 ``[rows]``, for the backward pass.  1 <= n <= 32768.
     ``out`` receives ``y`` and may be ``x``."""
-    _tensor(x, "x", 2)
+    dev = _device_of(x, "x")
+    rows, n, ldx = _matrix(x, "x", None, dev)
     dtype, device = x.dtype, x.device
-    rows, n = x.shape
     if not 1 <= n <= 32768:
         raise ValueError("layer norm takes 1 to 32768 columns, got %d" % n)
     if not eps >= 0.0:
         raise ValueError("eps must be >= 0, got %r" % (eps,))
-    w_f32 = _norm_weight(weight, bias, dtype, device, n)
-    if out is not None:
-        _tensor(out, "out", 2, dtype, device)
-        _shape(out, "out", (rows, n))
-    ldx = _ld(x, "x")
-    _on_gpu(x)
-    y = torch.empty((rows, n), dtype=dtype, device=device) if out is None else out
-    stats = torch.empty((2, rows), dtype=torch.float32, device=device)
-    mean, rstd = stats.unbind(0)
-    args = _hip.LayerNorm(_DTYPES[dtype], w_f32, rows, n, eps, x.data_ptr(), ldx, None, 0, None if weight is None else weight.data_ptr(),
-                          None if bias is None else bias.data_ptr(), y.data_ptr(), _ld(y, "out"), mean.data_ptr(), rstd.data_ptr())
-    _call(device, _hip.load().smrt_layer_norm_forward, "smrt_layer_norm_forward", C.byref(args))
+    w_f32, w_ptr, b_ptr = _norm_weight(weight, bias, dtype, dev, n)
+    if out is None:
+        _on_gpu(dev)
+        y, ldy = torch.empty((rows, n), dtype=dtype, device=device), n
+    else:
+        y_rows, y_cols, ldy = _matrix(out, "out", dtype, dev)
+        if y_rows != rows or y_cols != n:
+            _shape(out, "out", (rows, n))
+        _on_gpu(dev)
+        y = out
+    mean = torch.empty((rows,), dtype=torch.float32, device=device)
+    rstd = torch.empty((rows,), dtype=torch.float32, device=device)
+    args = _hip.LayerNorm(_DTYPES[dtype], w_f32, rows, n, eps, x.data_ptr(), ldx, None, 0, w_ptr, b_ptr, y.data_ptr(), ldy, mean.data_ptr(), rstd.data_ptr())
+    _call(dev, _hip.load().smrt_layer_norm_forward, C.byref(args))
     return y, mean, rstd
 
 
 def layer_norm_backward(grad, x, mean, rstd, weight=None, need_x=True, need_weight=True, need_bias=True):
     """Gradients ``(dx, dweight, dbias)`` of ``layer_norm`` from ``grad`` = d loss / d y.  ``x`` is the forward pass's input or its 8-bit form;
     ``mean`` and ``rstd`` are what it returned.  Without a ``weight`` only ``dx`` is computed."""
-    _tensor(grad, "grad", 2)
+    dev = _device_of(grad, "grad")
+    rows, n, ldg = _matrix(grad, "grad", None, dev)
     dtype, device = grad.dtype, grad.device
-    rows, n = grad.shape
     if not 1 <= n <= 32768:
         raise ValueError("layer norm takes 1 to 32768 columns, got %d" % n)
-    w_f32 = _norm_weight(weight, None, dtype, device, n)
-    x_ptr, ldx, xs_ptr, ld_xs = _kept(x, "x", (rows, n), dtype, device)
-    for t, name in ((mean, "mean"), (rstd, "rstd")):
-        _tensor(t, name, 1, torch.float32, device)
-        _shape(t, name, (rows,))
-    need_weight, need_bias = need_weight and weight is not None, need_bias and weight is not None
-    ldg = _ld(grad, "grad")
-    _on_gpu(grad)
+    w_f32, w_ptr, _ = _norm_weight(weight, None, dtype, dev, n)
+    x_ptr, ldx, xs_ptr, ld_xs = _kept(x, "x", rows, n, dtype, dev)
+    _tensor(mean, "mean", 1, torch.float32, dev)
+    _tensor(rstd, "rstd", 1, torch.float32, dev)
+    if mean.shape[0] != rows or rstd.shape[0] != rows:
+        raise ValueError("mean and rstd must have shape (%d,), got %r and %r" % (rows, tuple(mean.shape), tuple(rstd.shape)))
+    _on_gpu(dev)
     dx = torch.empty((rows, n), dtype=dtype, device=device) if need_x else None
-    dw = torch.empty((n,), dtype=weight.dtype, device=device) if need_weight else None
-    db = torch.empty((n,), dtype=weight.dtype, device=device) if need_bias else None
-    args = _hip.LayerNorm(_DTYPES[dtype], w_f32, rows, n, 0.0, x_ptr, ldx, xs_ptr, ld_xs, None if weight is None else weight.data_ptr(), None,
-                          None, 0, mean.data_ptr(), rstd.data_ptr(), grad.data_ptr(), ldg, dx.data_ptr() if need_x else None, n,
-                          dw.data_ptr() if need_weight else None, db.data_ptr() if need_bias else None)
+    dw = torch.empty((n,), dtype=weight.dtype, device=device) if need_weight and weight is not None else None
+    db = torch.empty((n,), dtype=weight.dtype, device=device) if need_bias and weight is not None else None
+    args = _hip.LayerNorm(_DTYPES[dtype], w_f32, rows, n, 0.0, x_ptr, ldx, xs_ptr, ld_xs, w_ptr, None, None, 0, mean.data_ptr(), rstd.data_ptr(),
+                          grad.data_ptr(), ldg, None if dx is None else dx.data_ptr(), n, None if dw is None else dw.data_ptr(),
+                          None if db is None else db.data_ptr())
     lib, ref = _hip.load(), C.byref(args)
     size = lib.smrt_layer_norm_backward_workspace(ref)
-    work = torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
-    _call(device, lib.smrt_layer_norm_backward, "smrt_layer_norm_backward", ref, None if work is None else work.data_ptr(), max(size, 0))
+    work = torch.empty((size,), dtype=torch.uint8, device=device) if size > 0 else None
+    _call(dev, lib.smrt_layer_norm_backward, ref, None if work is None else work.data_ptr(), size)
     return dx, dw, db

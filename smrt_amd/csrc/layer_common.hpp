@@ -54,23 +54,23 @@ template <class T> __device__ __forceinline__ void store8f(T* p, int valid, cons
 
 // Activations.  Unlike act_fwd these hand a NaN on (relu of the training kernels is fmaxf, which drops it: there the loss
 // reports it; here the value is the user's).
-__device__ __forceinline__ void layer_act8(int act, float (&v)[8]) {
+template <int N> __device__ __forceinline__ void layer_act(int act, float* v) {
     switch (act) {
         case ACT_SIGMOID:
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = fast_sigmoid(v[j]);
+            for (int j = 0; j < N; ++j) v[j] = fast_sigmoid(v[j]);
             break;
         case ACT_TANH:
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = tanhf(v[j]);
+            for (int j = 0; j < N; ++j) v[j] = tanhf(v[j]);
             break;
         case ACT_RELU:
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];
+            for (int j = 0; j < N; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];
             break;
         case ACT_ELU:
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = v[j] > 0.0f ? v[j] : expm1f(v[j]);
+            for (int j = 0; j < N; ++j) v[j] = v[j] > 0.0f ? v[j] : expm1f(v[j]);
             break;
         default: break;
     }

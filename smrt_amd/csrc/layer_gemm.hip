@@ -5,8 +5,8 @@
 namespace smrt {
 namespace layers {
 
-template <class T, int LAYOUT, bool PACKED> static hipError_t run(const GemmArgs& in, hipStream_t stream) {
-    constexpr int BM = 128, BN = 128, BK = sizeof(T) == 4 ? 32 : 64;
+template <class T, int LAYOUT, bool PACKED, int BM, int BN, int BK, int WAVES_M, int WAVES_N, int WAVES_K, int BUFS>
+static hipError_t run(const GemmArgs& in, hipStream_t stream) {
     GemmArgs g = in;
     g.tiles_n = (g.N + BN - 1) / BN;
     const int64_t tiles_m = LAYOUT == LAYOUT_DW ? (int64_t)((g.M + BM - 1) / BM) * g.groups * g.splits
@@ -15,14 +15,28 @@ template <class T, int LAYOUT, bool PACKED> static hipError_t run(const GemmArgs
     const int64_t blocks = tiles_m * g.tiles_n;
     if (blocks <= 0) return hipSuccess;
     if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((layer_gemm_kernel<T, LAYOUT, PACKED, BM, BN, BK, 2, 2>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
+    hipLaunchKernelGGL((layer_gemm_kernel<T, LAYOUT, PACKED, BM, BN, BK, WAVES_M, WAVES_N, WAVES_K, BUFS>), dim3((unsigned)blocks),
+                       dim3(WAVES_M * WAVES_N * WAVES_K * 64), 0, stream, g);
     return hipGetLastError();
 }
 
-hipError_t LAYER_NAME(int layout, const GemmArgs& g, hipStream_t stream) {
-    if (layout == LAYOUT_FORWARD) return run<LAYER_T, LAYOUT_FORWARD, false>(g, stream);
-    if (layout == LAYOUT_DX) return run<LAYER_T, LAYOUT_DX, false>(g, stream);
-    return g.A_scale ? run<LAYER_T, LAYOUT_DW, true>(g, stream) : run<LAYER_T, LAYOUT_DW, false>(g, stream);
+template <class T, int LAYOUT, bool PACKED> static hipError_t run_tile(int tile, const GemmArgs& g, hipStream_t stream) {
+    if constexpr (sizeof(T) == 4) {
+        if (tile == TILE_SMALL) return run<T, LAYOUT, PACKED, 64, 64, 64, 1, 1, 4, 1>(g, stream);
+        return run<T, LAYOUT, PACKED, 128, 128, 32, 2, 2, 1, 1>(g, stream);
+    } else {
+        // 256x256: steps of 64 where both operands lie along the summed index (dx: 153 us against 157 at 65536 x 1024 x 1024), of 32
+        // where one is turned (forward: 165 against 180)
+        if (tile == TILE_LARGE) return run<T, LAYOUT, PACKED, 256, 256, LAYOUT == LAYOUT_DX ? 64 : 32, 2, 4, 1, 2>(g, stream);
+        if (tile == TILE_MEDIUM) return run<T, LAYOUT, PACKED, 128, 128, 64, 2, 2, 1, 2>(g, stream);
+        return run<T, LAYOUT, PACKED, 64, 64, 128, 1, 1, 4, 2>(g, stream);
+    }
+}
+
+hipError_t LAYER_NAME(int layout, const GemmPlan& p, const GemmArgs& g, hipStream_t stream) {
+    if (layout == LAYOUT_FORWARD) return run_tile<LAYER_T, LAYOUT_FORWARD, false>(p.tile, g, stream);
+    if (layout == LAYOUT_DX) return run_tile<LAYER_T, LAYOUT_DX, false>(p.tile, g, stream);
+    return g.A_scale ? run_tile<LAYER_T, LAYOUT_DW, true>(p.tile, g, stream) : run_tile<LAYER_T, LAYOUT_DW, false>(p.tile, g, stream);
 }
 
 }  // namespace layers

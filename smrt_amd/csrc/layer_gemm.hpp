@@ -44,14 +44,13 @@ __device__ __forceinline__ uint32_t pack_hi(float a, float b) {     // the upper
 }
 
 // ---- staging.  A tile is ROWS x COLS elements of a row-major matrix, moved in pieces of 8 columns.  In LDS a row keeps its
-// order but its pieces are exchanged by an XOR with row bits, so that the lanes that one LDS cycle serves meet all banks:
-// along the summed index (READ_ALONG) 8 rows x one piece, across it 4 rows x 32 bytes.
+// order but its pieces are exchanged by an XOR with row bits, so that the lanes that one LDS cycle serves (256 bytes) meet all
+// 64 banks: along the summed index (ALONG) 16 rows x one piece, across it 4 rows x 64 bytes.
 template <int COLS, bool ALONG> struct Swizzle {
     static constexpr int CH = COLS / 8;
     __device__ static __forceinline__ int at(int row, int piece) {
         if (ALONG) {
-            constexpr int per = CH >= 8 ? 1 : 8 / CH;
-            constexpr int mask = CH >= 8 ? 7 : CH - 1;
+            constexpr int per = CH >= 16 ? 1 : 16 / CH, mask = CH >= 16 ? 15 : CH - 1;
             return row * CH + (piece ^ ((row / per) & mask));
         }
         return CH >= 16 ? row * CH + (piece ^ ((row & 3) << 2)) : row * CH + (piece ^ (((row >> 1) & 1) << 2));
@@ -63,37 +62,89 @@ template <> struct Raw<float, false> { u32x4 v[2]; };
 template <class T> struct Raw<T, true> { u32x2 q; uint32_t scale; };
 
 template <class T, bool PACKED, int ROWS, int COLS, int THREADS, bool ALONG> struct Stage {
-    static constexpr int PIECES = ROWS * COLS / 8;
-    static constexpr int PER = PIECES / THREADS;
+    static constexpr int CH = COLS / 8, PIECES = ROWS * CH, PER = PIECES / THREADS, STEP = THREADS / CH;
     static constexpr int PLANES = PACKED ? 1 : Planes<T>::n;
+    static constexpr int ESZ = PACKED ? 1 : sizeof(T);
     typedef typename Planes<T>::half half;
-    static_assert(PIECES % THREADS == 0, "pieces of a tile over the threads");
+    static_assert(PIECES % THREADS == 0 && THREADS % CH == 0, "a thread keeps its columns");
     Raw<T, PACKED> raw[PER];
+    uint32_t off[PER], soff[PACKED ? PER : 1];       // bytes from the tile's first element (of the scale bytes)
+    int shift;                                       // across: elements by which the piece that the row's end cuts is read earlier
 
-    // rows [row0, row_end), columns [col0, col_end) of the matrix; what lies outside is zero
-    __device__ __forceinline__ void load(const void* base, int64_t ld, const uint8_t* scale, int64_t ld_scale, int row0, int row_end,
-                                         int col0, int col_end) {
+    // rows and cols: what the tile has of the matrix along its own index (rows for ALONG, columns otherwise).  Everything else
+    // that a thread loads lies inside for every whole step along the summed index, so those loads need no test: rows behind the
+    // end read the last row and columns behind the end the last ones, which only reaches results that are never stored.
+    // back: how many columns before the tile's first the loads' base lies (a piece read earlier may begin there).
+    __device__ __forceinline__ void init(int64_t ld, int64_t ld_scale, int rows, int cols, int back) {
+        const int row = threadIdx.x / CH;
+        int col = (threadIdx.x % CH) * 8;
+        shift = 0;
+        if (!ALONG && col + 8 > cols) {
+            const int c = PACKED ? (cols - 1) & -8 : cols - 8;
+            shift = col < cols ? col - c : 0;
+            col = c;
+        }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int p = threadIdx.x + i * THREADS, row = row0 + p / (COLS / 8), col = col0 + (p % (COLS / 8)) * 8;
-            const int valid = row < row_end ? col_end - col : 0;
+            int r = row + i * STEP;
+            if (ALONG) r = r < rows ? r : rows - 1;
+            off[i] = (uint32_t)r * (uint32_t)ld * ESZ + (uint32_t)(col + back) * ESZ;
+            if constexpr (PACKED) soff[i] = (uint32_t)r * (uint32_t)ld_scale + (uint32_t)col / PACK_BLOCK;
+        }
+    }
+    // a whole step; base (and scale) are the same in all lanes
+    __device__ __forceinline__ void load(const char* base, const uint8_t* scale) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if constexpr (PACKED) {
+                __builtin_memcpy(&raw[i].q, base + off[i], 8);
+                raw[i].scale = scale[soff[i]];
+            } else {
+                const T* src = (const T*)(base + off[i]);
+                __builtin_memcpy(&raw[i], src, 8 * sizeof(T));
+            }
+        }
+    }
+    // the piece that was read `shift` elements early, moved to its place (what comes in behind it is never used)
+    __device__ __forceinline__ void unshift() {
+        if constexpr (!ALONG && !PACKED) {
+            constexpr int W = 2 * sizeof(T);         // words of a piece
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                uint32_t w[W];
+                __builtin_memcpy(w, &raw[i], 4 * W);
+#pragma unroll
+                for (int step = 4; step >= 1; step >>= 1) {
+                    const bool on = shift & step;
+                    if (sizeof(T) == 2 && step == 1) {
+#pragma unroll
+                        for (int j = 0; j < W; ++j) w[j] = on ? __builtin_amdgcn_alignbit(j + 1 < W ? w[j + 1] : 0u, w[j], 16) : w[j];
+                    } else {
+                        const int by = step * (int)sizeof(T) / 4;
+#pragma unroll
+                        for (int j = 0; j < W; ++j) w[j] = on ? (j + by < W ? w[j + by] : 0u) : w[j];
+                    }
+                }
+                __builtin_memcpy(&raw[i], w, 4 * W);
+            }
+        }
+    }
+    // the last step along the summed index, with tests: rows x cols is what there is of the tile, the rest is zero
+    __device__ __forceinline__ void load_tail(const char* base, const uint8_t* scale, int64_t ld, int64_t ld_scale, int rows, int cols) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int row = threadIdx.x / CH + i * STEP, col = (threadIdx.x % CH) * 8, valid = row < rows ? cols - col : 0;
             if constexpr (PACKED) {
                 raw[i].q = u32x2{0u, 0u};
                 raw[i].scale = 0u;
-                if (valid > 0) {                 // the 8-bit rows are padded to whole blocks with zeros
-                    __builtin_memcpy(&raw[i].q, (const int8_t*)base + (int64_t)row * ld + col, 8);
+                if (valid > 0) {                     // the 8-bit rows are padded to whole blocks with zeros
+                    __builtin_memcpy(&raw[i].q, base + (int64_t)row * ld + col, 8);
                     raw[i].scale = scale[(int64_t)row * ld_scale + col / PACK_BLOCK];
                 }
             } else {
-                const T* src = (const T*)base + (int64_t)row * ld + col;
-                if (valid >= 8) {
-                    __builtin_memcpy(&raw[i], src, 8 * sizeof(T));
-                } else {
-                    T v[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = j < valid ? src[j] : (T)0.0f;
-                    __builtin_memcpy(&raw[i], v, 8 * sizeof(T));
-                }
+                T v[8];
+                load8((const T*)base + (int64_t)row * ld + col, valid, v);
+                __builtin_memcpy(&raw[i], v, 8 * sizeof(T));
             }
         }
     }
@@ -101,8 +152,7 @@ template <class T, bool PACKED, int ROWS, int COLS, int THREADS, bool ALONG> str
     __device__ __forceinline__ void store(half* lds) const {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int p = threadIdx.x + i * THREADS;
-            u32x4* dst = (u32x4*)lds + Swizzle<COLS, ALONG>::at(p / (COLS / 8), p % (COLS / 8));
+            u32x4* dst = (u32x4*)lds + Swizzle<COLS, ALONG>::at(threadIdx.x / CH + i * STEP, threadIdx.x % CH);
             if constexpr (PACKED) {
                 float f[8];
                 unpack8(raw[i].q, unpack_scale((int)raw[i].scale), f);
@@ -168,10 +218,21 @@ __device__ __forceinline__ int xcd_tile(int b, int total) {
     return x * per + (x < rest ? x : rest) + i;
 }
 
-template <class T, int LAYOUT, bool PACKED_A, int BM, int BN, int BK, int WAVES_M, int WAVES_N>
-__global__ void __launch_bounds__(WAVES_M * WAVES_N * 64, 2) layer_gemm_kernel(GemmArgs g) {
-    constexpr int THREADS = WAVES_M * WAVES_N * 64;
-    constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 32, NI = WN / 32;
+// All waves have written their part of LDS and read what they needed.  Loads from global memory go on.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// BUFS = 2: while one step of BK is multiplied the next goes from registers into the other half of LDS and the one after
+// it is requested from memory; one barrier a step.  BUFS = 1 (fp32, whose three parts fill LDS): two barriers a step, and the
+// other workgroup of the CU multiplies meanwhile.
+// WAVES_K > 1: the waves share a small tile and split each step's summed indices between them; their sums are joined in LDS.
+template <class T, int LAYOUT, bool PACKED_A, int BM, int BN, int BK, int WAVES_M, int WAVES_N, int WAVES_K, int BUFS>
+__global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gemm_kernel(GemmArgs g) {
+    constexpr int WAVES = WAVES_M * WAVES_N * WAVES_K, THREADS = WAVES * 64;
+    constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 32, NI = WN / 32, KS = BK / 16 / WAVES_K;
     constexpr bool SPLIT3 = Planes<T>::n == 3;
     constexpr bool A_ALONG = LAYOUT != LAYOUT_DW, B_ALONG = LAYOUT == LAYOUT_DX;
     typedef typename Planes<T>::half half;
@@ -179,15 +240,14 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * 64, 2) layer_gemm_kernel(G
     typedef Stage<T, PACKED_A, A_ALONG ? BM : BK, A_ALONG ? BK : BM, THREADS, A_ALONG> StageA;
     typedef Stage<T, false, B_ALONG ? BN : BK, B_ALONG ? BK : BN, THREADS, B_ALONG> StageB;
     constexpr int PA = StageA::PLANES, PB = StageB::PLANES;
-    constexpr int LDS_A = PA * BM * BK, LDS_B = PB * BN * BK;
-    constexpr int EPI_LD = WN + 4;
-    constexpr int EPI = WAVES_M * WAVES_N * 32 * EPI_LD * 4, MAIN = (LDS_A + LDS_B) * 2;
+    constexpr int LDS_A = PA * BM * BK, LDS_B = PB * BN * BK, LDS_STEP = LDS_A + LDS_B;
+    constexpr int EPI_LD = WN + 4, EPI_ROWS = WAVES_K > 1 ? WM : 32;
+    constexpr int EPI = WAVES * EPI_ROWS * EPI_LD * 4, MAIN = LDS_STEP * 2 * BUFS;
     __shared__ __attribute__((aligned(16))) char smem[EPI > MAIN ? EPI : MAIN];
-    half* const lds_a = (half*)smem;
-    half* const lds_b = lds_a + LDS_A;
+    half* const lds = (half*)smem;
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = (wave / WAVES_N) * WM, wn = (wave % WAVES_N) * WN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wk = wave / (WAVES_M * WAVES_N), wm = (wave / WAVES_N % WAVES_M) * WM, wn = (wave % WAVES_N) * WN;
 
     // which tile, of which group
     int bid = xcd_tile(blockIdx.x, gridDim.x);
@@ -202,7 +262,11 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * 64, 2) layer_gemm_kernel(G
         group = bid % g.groups;
         slice = bid / g.groups;
         int r0 = 0, r1 = g.rows;
-        if (g.ends) { const RowSpan s = group_rows(g.ends, group, g.rows); r0 = s.r0; r1 = s.r1; }
+        if (g.ends) {
+            const RowSpan s = group_rows(g.ends, group, g.rows);
+            r0 = __builtin_amdgcn_readfirstlane(s.r0);
+            r1 = __builtin_amdgcn_readfirstlane(s.r1);
+        }
         int per = (r1 - r0 + g.splits - 1) / g.splits;
         per = (per + BK - 1) / BK * BK;
         const long b0 = r0 + (long)slice * per;
@@ -211,7 +275,9 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * 64, 2) layer_gemm_kernel(G
     } else {
         if (g.ends) {
             const RowSpan s = tile_rows(g.ends, g.groups, g.rows, bid, BM);
-            group = s.group; m0 = s.r0; m_end = s.r1;
+            group = __builtin_amdgcn_readfirstlane(s.group);
+            m0 = __builtin_amdgcn_readfirstlane(s.r0);
+            m_end = __builtin_amdgcn_readfirstlane(s.r1);
             if (m0 >= m_end) return;
         } else {
             m0 = bid * BM;
@@ -223,118 +289,212 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * 64, 2) layer_gemm_kernel(G
     if (rest) k_end = k0;
 
     f32x16 acc[MI][NI] = {}, low[SPLIT3 ? MI : 1][SPLIT3 ? NI : 1] = {};
-    const char* Bg = (const char*)g.B;
-    if (LAYOUT != LAYOUT_DW) Bg += (int64_t)(rest ? 0 : group) * g.strideB * (int64_t)sizeof(T);
-
     StageA sa;
     StageB sb;
-    auto fetch = [&](int k) {
-        if constexpr (A_ALONG) sa.load(g.A, g.lda, g.A_scale, g.lds_scale, m0, m_end, k, k_end);
-        else                   sa.load(g.A, g.lda, g.A_scale, g.lds_scale, k, k_end, m0, m_end);
-        if constexpr (B_ALONG) sb.load(Bg, g.ldb, nullptr, 0, n0, g.N, k, k_end);
-        else                   sb.load(Bg, g.ldb, nullptr, 0, k, k_end, n0, g.N);
+    // the tiles' first elements, and how far a step along the summed index is
+    const int64_t esa = StageA::ESZ, esb = sizeof(T);
+    const char* pa = (const char*)g.A + (A_ALONG ? m0 * g.lda + k0 : k0 * g.lda + m0) * esa;
+    const uint8_t* psc = PACKED_A ? g.A_scale + (int64_t)k0 * g.lds_scale + m0 / PACK_BLOCK : nullptr;
+    const char* pb = (const char*)g.B + ((LAYOUT == LAYOUT_DW || rest ? 0 : group) * g.strideB + (B_ALONG ? n0 * g.ldb + k0 : k0 * g.ldb + n0)) * esb;
+    const int64_t step_a = (A_ALONG ? BK : BK * g.lda) * esa, step_b = (B_ALONG ? BK : BK * g.ldb) * esb, step_sc = PACKED_A ? BK * g.lds_scale : 0;
+    const int m_has = m_end - m0, n_has = g.N - n0;
+    const bool edge_a = !A_ALONG && !PACKED_A && m_has < BM && (m_has & 7), edge_b = !B_ALONG && n_has < BN && (n_has & 7);
+    const int back_a = A_ALONG || PACKED_A || m0 == 0 ? 0 : 8, back_b = B_ALONG || n0 == 0 ? 0 : 8;
+    pa -= back_a * esa;
+    pb -= back_b * esb;
+    // a matrix of fewer than 8 columns has no whole piece: every step is then loaded with tests
+    const int whole = (!A_ALONG && !PACKED_A && g.M < 8) || (!B_ALONG && g.N < 8) ? 0 : (k_end - k0) / BK;
+    sa.init(g.lda, g.lds_scale, m_has, m_has, back_a);
+    sb.init(g.ldb, 0, n_has, n_has, back_b);
+    const int steps = (k_end - k0 + BK - 1) / BK;
+    auto fetch = [&](int t) {
+        if (t < whole) {
+            sa.load(pa, psc);
+            sb.load(pb, nullptr);
+        } else {
+            const int k_has = k_end - k0 - t * BK;
+            sa.load_tail(pa + back_a * esa, psc, g.lda, g.lds_scale, A_ALONG ? m_has : k_has, A_ALONG ? k_has : m_has);
+            sb.load_tail(pb + back_b * esb, nullptr, g.ldb, 0, B_ALONG ? n_has : k_has, B_ALONG ? k_has : n_has);
+        }
+        pa += step_a;
+        pb += step_b;
+        if (PACKED_A) psc += step_sc;
     };
-    if (k0 < k_end) fetch(k0);
-    for (int k = k0; k < k_end; k += BK) {
-        __syncthreads();
-        sa.store(lds_a);
-        sb.store(lds_b);
-        __syncthreads();
-        if (k + BK < k_end) fetch(k + BK);
+    auto put = [&](int t, half* to) {
+        if (t < whole) {
+            if (edge_a) sa.unshift();
+            if (edge_b) sb.unshift();
+        }
+        sa.store(to);
+        sb.store(to + LDS_A);
+    };
+    frag fa[2][PA][MI], fb[2][PB][NI];
+    auto read = [&](const half* from, int ks) {
+        frag (&a)[PA][MI] = fa[ks & 1];
+        frag (&b)[PB][NI] = fb[ks & 1];
 #pragma unroll
-        for (int ks = 0; ks < BK / 16; ++ks) {
-            frag fa[PA][MI], fb[PB][NI];
+        for (int p = 0; p < PA; ++p)
 #pragma unroll
-            for (int p = 0; p < PA; ++p)
+            for (int i = 0; i < MI; ++i) a[p][i] = read_frag<half, A_ALONG ? BK : BM, A_ALONG>(from + p * BM * BK, wm + i * 32, wk * KS + ks, lane);
 #pragma unroll
-                for (int i = 0; i < MI; ++i) fa[p][i] = read_frag<half, A_ALONG ? BK : BM, A_ALONG>(lds_a + p * BM * BK, wm + i * 32, ks, lane);
+        for (int p = 0; p < PB; ++p)
 #pragma unroll
-            for (int p = 0; p < PB; ++p)
+            for (int j = 0; j < NI; ++j) b[p][j] = read_frag<half, B_ALONG ? BK : BN, B_ALONG>(from + LDS_A + p * BN * BK, wn + j * 32, wk * KS + ks, lane);
+    };
+    auto multiply = [&](int ks) {
+        frag (&a)[PA][MI] = fa[ks & 1];
+        frag (&b)[PB][NI] = fb[ks & 1];
 #pragma unroll
-                for (int j = 0; j < NI; ++j) fb[p][j] = read_frag<half, B_ALONG ? BK : BN, B_ALONG>(lds_b + p * BN * BK, wn + j * 32, ks, lane);
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
+            for (int j = 0; j < NI; ++j) {
+                if constexpr (SPLIT3) {
 #pragma unroll
-                for (int j = 0; j < NI; ++j) {
-                    if constexpr (SPLIT3) {
+                    for (int s = 2; s >= 1; --s)                              // smallest terms first
 #pragma unroll
-                        for (int s = 2; s >= 1; --s)                      // smallest terms first
-#pragma unroll
-                            for (int p = 0; p <= s; ++p)
-                                if (p < PA && s - p < PB) low[i][j] = Mfma<half>::mul(fa[p][i], fb[s - p][j], low[i][j]);
-                    }
-                    acc[i][j] = Mfma<half>::mul(fa[0][i], fb[0][j], acc[i][j]);
+                        for (int p = 0; p <= s; ++p)
+                            if (p < PA && s - p < PB) low[i][j] = Mfma<half>::mul(a[p][i], b[s - p][j], low[i][j]);
                 }
+                acc[i][j] = Mfma<half>::mul(a[0][i], b[0][j], acc[i][j]);
+            }
+    };
+    if constexpr (BUFS == 1) {
+        if (steps) fetch(0);
+        for (int t = 0; t < steps; ++t) {
+            lds_barrier();
+            put(t, lds);
+            lds_barrier();
+            if (t + 1 < steps) fetch(t + 1);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) { read(lds, ks); multiply(ks); }
+        }
+    } else {
+        if (steps) { fetch(0); put(0, lds); }
+        if (steps > 1) fetch(1);
+        for (int t = 0; t < steps; ++t) {
+            const half* cur = lds + (t & 1) * LDS_STEP;
+            lds_barrier();
+            read(cur, 0);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks + 1 < KS) read(cur, ks + 1);
+                multiply(ks);
+                if (ks == 0 && t + 1 < steps) {
+                    put(t + 1, lds + ((t + 1) & 1) * LDS_STEP);
+                    if (t + 2 < steps) fetch(t + 2);
+                }
+            }
         }
     }
-    __syncthreads();
 
-    // ---- epilogue: 32 rows of the wave's tile at a time through LDS, so that a lane ends up with 8 columns of a row
-    float* const tile = (float*)smem + wave * 32 * EPI_LD;
-    const int64_t out0 = LAYOUT == LAYOUT_DW ? (int64_t)group * g.strideC : 0;
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+    // ---- epilogue: 32 rows of the wave's tile at a time through LDS, so that a lane ends up with 8 columns of a row, the same
+    // ones for all its rows.  What it reads besides (bias, residual) is requested two passes ahead, into the registers that the
+    // operands have left.
+    // With WAVES_K > 1 every wave puts its sums of the whole tile there, and takes a share of the rows.
+    constexpr int PASS_ROWS = WAVES_K > 1 ? WM / WAVES_K : 32, PASSES = WAVES_K > 1 ? 1 : MI;
+    constexpr int ROWP = WN / 8, STEPS = PASS_ROWS * ROWP / 64, ROWS_PER = 64 / ROWP;
+    static_assert(64 % ROWP == 0 && STEPS > 0 && (WAVES_K == 1 || WAVES_M * WAVES_N == 1), "a lane keeps its columns");
+    auto put_sums = [&](int i, float* to) {
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 float v = acc[i][j][r];
                 if constexpr (SPLIT3) { const float w = v + low[i][j][r]; v = __builtin_isfinite(v) ? w : v; }
-                tile[((r >> 2) * 8 + (lane >> 5) * 4 + (r & 3)) * EPI_LD + j * 32 + (lane & 31)] = v;
+                to[((r >> 2) * 8 + (lane >> 5) * 4 + (r & 3)) * EPI_LD + j * 32 + (lane & 31)] = v;
             }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-        for (int it = 0; it < 32 * WN / 8 / 64; ++it) {
-            const int p = it * 64 + lane, tr = p / (WN / 8), col = n0 + wn + (p % (WN / 8)) * 8;
-            const int row = m0 + wm + i * 32 + tr;
-            const int valid = row < m_end ? g.N - col : 0;
-            float v[8];
+    };
+    float* const tile = (float*)smem + wave * EPI_ROWS * EPI_LD;
+    const int ccol = (lane % ROWP) * 8, col = n0 + wn + ccol, cvalid = g.N - col;
+    float bias[8] = {};
+    if constexpr (LAYOUT == LAYOUT_FORWARD) {
+        if (g.bias && !rest && cvalid > 0) load8f((const T*)g.bias + (int64_t)group * g.stride_bias + col, cvalid, bias);
+    }
+    const int row_first = m0 + (WAVES_K > 1 ? wk * PASS_ROWS : wm) + lane / ROWP;
+    T res[2][STEPS][8];
+    auto fetch_residual = [&](int i) {
+        if constexpr (LAYOUT == LAYOUT_FORWARD) {
+            if (g.residual && !rest && i < PASSES) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const f32x4 w = *(const f32x4*)(tile + tr * EPI_LD + (p % (WN / 8)) * 8 + 4 * h);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[4 * h + j] = w[j];
+                for (int it = 0; it < STEPS; ++it) {
+                    const int row = row_first + i * 32 + it * ROWS_PER;
+                    load8((const T*)g.residual + (int64_t)row * g.ldr + col, row < m_end ? cvalid : 0, res[i & 1][it]);
+                }
             }
+        }
+    };
+    fetch_residual(0);
+    fetch_residual(1);
+    __syncthreads();
+    if constexpr (WAVES_K > 1) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) put_sums(i, tile + i * 32 * EPI_LD);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const int row0 = row_first + i * 32;
+        if constexpr (WAVES_K == 1) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            put_sums(i, tile);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+        float v[STEPS][8] = {};
+#pragma unroll
+        for (int it = 0; it < STEPS; ++it)
+#pragma unroll
+            for (int w = 0; w < WAVES_K; ++w) {
+                const float* from = WAVES_K > 1 ? (const float*)smem + (w * EPI_ROWS + wk * PASS_ROWS) * EPI_LD : tile;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const f32x4 s = *(const f32x4*)(from + (it * ROWS_PER + lane / ROWP) * EPI_LD + ccol + 4 * h);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[it][4 * h + j] += s[j];
+                }
+            }
+        if constexpr (LAYOUT == LAYOUT_FORWARD) {
+#pragma unroll
+            for (int it = 0; it < STEPS; ++it)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[it][j] += bias[j];
+            layer_act<STEPS * 8>(g.act, &v[0][0]);
+            if (rest) {
+#pragma unroll
+                for (int it = 0; it < STEPS; ++it)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[it][j] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int it = 0; it < STEPS; ++it) {
+            const int row = row0 + it * ROWS_PER, valid = row < m_end ? cvalid : 0;
             if constexpr (LAYOUT == LAYOUT_DW) {
                 if (valid <= 0) continue;
-                if (g.slab) store8(g.slab + (((int64_t)slice * g.groups + group) * g.M + row) * g.N + col, valid, v);
-                else        store8f((T*)g.C + out0 + (int64_t)row * g.ldc + col, valid, v);
+                if (g.slab) store8(g.slab + (((int64_t)slice * g.groups + group) * g.M + row) * g.N + col, valid, v[it]);
+                else        store8f((T*)g.C + (int64_t)group * g.strideC + (int64_t)row * g.ldc + col, valid, v[it]);
             } else if constexpr (LAYOUT == LAYOUT_DX) {
-                if (valid > 0 && !(rest && g.keep_rest)) store8f((T*)g.C + (int64_t)row * g.ldc + col, valid, v);
+                if (valid > 0 && !(rest && g.keep_rest)) store8f((T*)g.C + (int64_t)row * g.ldc + col, valid, v[it]);
             } else {
-                if (g.bias && !rest && valid > 0) {
-                    float b[8];
-                    load8f((const T*)g.bias + (int64_t)group * g.stride_bias + col, valid, b);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] += b[j];
-                }
-                layer_act8(g.act, v);
-                if (rest) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-                }
                 if (g.q_out) {
                     float a[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) a[j] = j < valid ? (float)(T)v[j] : 0.0f;      // the 8-bit form of the value in T
+                    for (int j = 0; j < 8; ++j) a[j] = j < valid ? (float)(T)v[it][j] : 0.0f;      // the 8-bit form of the value in T
                     pack_block<T>(a, lane, row < m_end && col < ((g.N + PACK_BLOCK - 1) & -PACK_BLOCK), g.q_out + (int64_t)row * g.ldq + col,
                                   g.q_scale + (int64_t)row * g.ldq_scale + col / PACK_BLOCK);
                 }
                 if (valid > 0) {
-                    if (g.act_out) store8f((T*)g.act_out + (int64_t)row * g.ld_act + col, valid, v);
+                    if (g.act_out) store8f((T*)g.act_out + (int64_t)row * g.ld_act + col, valid, v[it]);
                     if (g.residual && !rest) {
-                        float b[8];
-                        load8f((const T*)g.residual + (int64_t)row * g.ldr + col, valid, b);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) v[j] += b[j];
+                        for (int j = 0; j < 8; ++j) v[it][j] += (float)res[i & 1][it][j];
                     }
-                    if (!(rest && g.keep_rest)) store8f((T*)g.C + (int64_t)row * g.ldc + col, valid, v);
+                    if (!(rest && g.keep_rest)) store8f((T*)g.C + (int64_t)row * g.ldc + col, valid, v[it]);
                 }
             }
         }
+        fetch_residual(i + 2);
     }
 }
 

@@ -11,7 +11,7 @@ namespace smrt {
 namespace layers {
 namespace {
 
-constexpr int64_t MAX_ROWS = 0x7fffffff - 4096, MAX_COLS = 1 << 30;
+constexpr int64_t MAX_ROWS = 0x7fffffff - 4096, MAX_COLS = 1 << 30, MAX_LD = 1 << 21;     // a product tile of 256 rows spans less than 2^31 bytes
 constexpr int MAX_GROUPS = 65535;
 
 // ------------------------------------------------------------------------------------------------ dz = g * act'(a), column sums
@@ -336,6 +336,7 @@ int check_dense(const smrt_dense* p, const char* who) {
     if (p->groups < 1 || p->groups > MAX_GROUPS) return fail(who, "groups must be in [1, 65535]");
     if (p->groups > 1 && !p->ends) return fail(who, "more than one group needs ends");
     if (p->ldx < p->k || p->ldw < p->n) return fail(who, "a leading dimension is below its columns");
+    if (p->ldx > MAX_LD || p->ldw > MAX_LD || p->ldg > MAX_LD || p->ld_x_scale > MAX_LD) return fail(who, "a leading dimension is above 2^21");
     if (p->groups > 1 && p->w_stride < span(p->k, p->ldw, p->n)) return fail(who, "the groups' weights overlap");
     if (p->w_stride < 0) return fail(who, "bad sizes");
     if (p->groups > 1 && (p->bias || p->db) && p->bias_stride < p->n) return fail(who, "the groups' biases overlap");
@@ -344,13 +345,14 @@ int check_dense(const smrt_dense* p, const char* who) {
     return 0;
 }
 
-hipError_t gemm(int dtype, int layout, const GemmArgs& g, hipStream_t s) {
-    return dtype == SMRT_F32 ? layer_gemm_f32(layout, g, s) : dtype == SMRT_BF16 ? layer_gemm_bf16(layout, g, s) : layer_gemm_f16(layout, g, s);
+hipError_t gemm(int dtype, int layout, const GemmPlan& p, const GemmArgs& g, hipStream_t s) {
+    return dtype == SMRT_F32 ? layer_gemm_f32(layout, p, g, s) : dtype == SMRT_BF16 ? layer_gemm_bf16(layout, p, g, s) : layer_gemm_f16(layout, p, g, s);
 }
 
 struct BackwardPlan {
     bool need_dz, need_sum;
-    int dz_slices, splits;
+    int dz_slices;
+    GemmPlan dw;
     int64_t ld_dz, dz_bytes, slab_off, slab_bytes, part_off, part_bytes, total;
 };
 BackwardPlan plan_backward(const smrt_dense* p) {
@@ -364,9 +366,8 @@ BackwardPlan plan_backward(const smrt_dense* p) {
     // slices of a group's rows: enough workgroups for every CU several times over, none with fewer than 64 rows
     b.dz_slices = (int)std::max<int64_t>(1, std::min<int64_t>(avg / 64, 2048 / std::max<int64_t>(1, col_blocks * G)));
     b.part_bytes = b.need_sum && b.dz_slices > 1 ? pad((int64_t)b.dz_slices * G * p->n * 4, 256) : 0;
-    const int64_t tiles = ((p->k + 127) / 128) * ((p->n + 127) / 128) * G;
-    b.splits = p->dw ? (int)std::max<int64_t>(1, std::min<int64_t>(avg / 512, 512 / std::max<int64_t>(1, tiles))) : 1;
-    b.slab_bytes = p->dw && b.splits > 1 ? pad((int64_t)b.splits * G * p->k * p->n * 4, 256) : 0;
+    b.dw = plan_gemm(LAYOUT_DW, p->dtype == SMRT_F32, p->rows, p->k, p->n, G);
+    b.slab_bytes = p->dw && b.dw.splits > 1 ? pad((int64_t)b.dw.splits * G * p->k * p->n * 4, 256) : 0;
     b.slab_off = b.dz_bytes;
     b.part_off = b.slab_off + b.slab_bytes;
     b.total = b.part_off + b.part_bytes;
@@ -457,7 +458,7 @@ extern "C" int smrt_dense_forward(const smrt_dense* p, void* hip_stream) {
     else if (p->a) { g.act_out = p->a; g.ld_act = p->lda; }
     g.ends = p->ends; g.groups = p->groups; g.keep_rest = p->keep_rest; g.rows = (int32_t)p->rows;
     g.M = (int32_t)p->rows; g.N = (int32_t)p->n; g.K = (int32_t)p->k; g.splits = 1; g.act = p->activation;
-    return launched(who, gemm(p->dtype, LAYOUT_FORWARD, g, (hipStream_t)hip_stream));
+    return launched(who, gemm(p->dtype, LAYOUT_FORWARD, plan_gemm(LAYOUT_FORWARD, p->dtype == SMRT_F32, p->rows, p->rows, p->n, p->groups), g, (hipStream_t)hip_stream));
 }
 
 extern "C" int64_t smrt_dense_backward_workspace(const smrt_dense* p) {
@@ -501,18 +502,18 @@ extern "C" int smrt_dense_backward(const smrt_dense* p, void* workspace, int64_t
     if (p->dx && p->rows && p->k) {
         g.A = dz; g.lda = ld_dz; g.B = p->w; g.ldb = p->ldw; g.strideB = p->w_stride; g.C = p->dx; g.ldc = p->lddx;
         g.M = (int32_t)p->rows; g.N = (int32_t)p->k; g.K = (int32_t)p->n;
-        if (hipError_t e = gemm(p->dtype, LAYOUT_DX, g, stream); e != hipSuccess) return launched(who, e);
+        if (hipError_t e = gemm(p->dtype, LAYOUT_DX, plan_gemm(LAYOUT_DX, p->dtype == SMRT_F32, p->rows, p->rows, p->k, p->groups), g, stream); e != hipSuccess) return launched(who, e);
     }
     const bool dw = p->dw && p->k && p->n;
     if (dw) {
         g.A = p->x; g.lda = p->ldx; g.A_scale = p->x_scale; g.lds_scale = p->ld_x_scale; g.B = dz; g.ldb = ld_dz; g.strideB = 0;
         g.C = p->dw; g.ldc = p->lddw; g.strideC = p->dw_stride; g.slab = b.slab_bytes ? (float*)(ws + b.slab_off) : nullptr;
-        g.M = (int32_t)p->k; g.N = (int32_t)p->n; g.K = (int32_t)p->rows; g.splits = b.splits;
-        if (hipError_t e = gemm(p->dtype, LAYOUT_DW, g, stream); e != hipSuccess) return launched(who, e);
+        g.M = (int32_t)p->k; g.N = (int32_t)p->n; g.K = (int32_t)p->rows; g.splits = b.dw.splits;
+        if (hipError_t e = gemm(p->dtype, LAYOUT_DW, b.dw, g, stream); e != hipSuccess) return launched(who, e);
     }
     if ((dw && b.slab_bytes) || part) {
         JoinPart jw = {}, jb = {};
-        if (dw && b.slab_bytes) jw = join_part((const float*)(ws + b.slab_off), b.splits, p->groups * p->k * p->n, p->groups * p->k, p->n, p->dw, p->lddw, p->k, p->dw_stride, false, 1);
+        if (dw && b.slab_bytes) jw = join_part((const float*)(ws + b.slab_off), b.dw.splits, p->groups * p->k * p->n, p->groups * p->k, p->n, p->dw, p->lddw, p->k, p->dw_stride, false, 1);
         if (part && p->n) jb = join_part(part, b.dz_slices, p->groups * p->n, p->groups, p->n, p->db, 0, 1, p->bias_stride, false, 32);
         if (jw.blocks + jb.blocks) {
             const hipError_t e = by_type(p->dtype, [&](auto t) {

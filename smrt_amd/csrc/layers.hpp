@@ -1,11 +1,49 @@
-// Launchers of the layer products, one per element type (layer_gemm.hip).
+// The layer products' launchers, one per element type (layer_gemm.hip), and which tile shape a product gets.
 #pragma once
+#include <algorithm>
 #include "layer_gemm.hpp"
 
 namespace smrt {
 namespace layers {
-hipError_t layer_gemm_f32(int layout, const GemmArgs& g, hipStream_t stream);
-hipError_t layer_gemm_bf16(int layout, const GemmArgs& g, hipStream_t stream);
-hipError_t layer_gemm_f16(int layout, const GemmArgs& g, hipStream_t stream);
+
+enum Tile : int { TILE_LARGE = 0, TILE_MEDIUM = 1, TILE_SMALL = 2 };
+struct GemmPlan { int tile, splits; };
+
+// 16-bit types have 256x256 (8 waves, one workgroup a CU), 128x128 (4 waves, two a CU) and 64x64 tiles whose 4 waves split the
+// summed index; fp32, whose three parts fill the registers sooner, the last two.  A launch takes its share of rounds over the 256 CUs, and at
+// least as long as one tile's chain of loads and products.  Measured per 1024 summed indices, in us (one tile's chain | a round):
+//             16 bit: 256x256  30 | 40     128x128  18.5 | 11.7     64x64  10.5 | 5.6
+//             fp32:                        128x128  54   | 48       64x64  24   | 16
+// so 65536 x 1024 x 1024 in bf16 took 159 / 186 / 292 us on the three, 4096 x 1024 x 1024 36 / 22 / 25, 1024 x 784 x 450 32 / 21 / 13.
+inline GemmPlan plan_gemm(int layout, bool f32, int64_t rows, int64_t m, int64_t n, int64_t groups) {
+    constexpr int side[3] = {256, 128, 64};
+    constexpr double chain[2][3] = {{30, 18.5, 10.5}, {1e9, 54, 24}}, round[2][3] = {{40, 11.7, 5.6}, {1e9, 48, 16}};
+    GemmPlan best = {TILE_SMALL, 1};
+    double best_us = 1e30;
+    for (int t = f32 ? 1 : 0; t < 3; ++t) {
+        const int64_t tn = (n + side[t] - 1) / side[t];
+        GemmPlan p = {t, 1};
+        double us;
+        if (layout == LAYOUT_DW) {
+            // the weight gradient sums over the rows: few tiles, so a group's rows go to `splits` workgroups a tile, whose sums are
+            // joined afterwards (the slabs pass through memory twice)
+            const int64_t tiles = (m + side[t] - 1) / side[t] * tn * groups, avg = std::max<int64_t>(rows / groups, 1);
+            const int64_t want = (t == TILE_LARGE ? 256 : 512) / std::max<int64_t>(tiles, 1);
+            p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(avg / 512, want));
+            const double part = (double)avg / p.splits / 1024.0;
+            us = part * std::max(chain[f32][t], round[f32][t] * (double)((tiles * p.splits + 255) / 256));
+            if (p.splits > 1) us += 2.0 * p.splits * groups * m * n * 4.0 / 5e6;
+        } else {
+            const int64_t tiles = (groups == 1 ? (rows + side[t] - 1) / side[t] : rows / side[t] + groups / 2) * tn;     // about half a tile a group is empty
+            us = std::max(chain[f32][t], round[f32][t] * (double)((tiles + 255) / 256));
+        }
+        if (us < best_us) { best_us = us; best = p; }
+    }
+    return best;
+}
+
+hipError_t layer_gemm_f32(int layout, const GemmPlan& p, const GemmArgs& g, hipStream_t stream);
+hipError_t layer_gemm_bf16(int layout, const GemmPlan& p, const GemmArgs& g, hipStream_t stream);
+hipError_t layer_gemm_f16(int layout, const GemmPlan& p, const GemmArgs& g, hipStream_t stream);
 }  // namespace layers
 }  // namespace smrt

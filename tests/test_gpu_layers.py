@@ -585,3 +585,42 @@ def test_rows_past_32_bits():
     check_dense_backward(g, tail, w, None, "identity", dx[-64:], dw, db, BF16)
     assert torch.equal(layer_norm(x)[0][-64:], layer_norm(tail.cuda())[0])
     assert torch.equal(unpack_rows(pack_rows(x))[-64:], unpack_rows(pack_rows(tail.cuda())))
+
+
+TILES = [(16500, 100, 700), (70000, 40, 260), (5000, 300, 1030), (4200, 1032, 520), (3001, 515, 2050), (33000, 257, 263)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("i", range(len(TILES)), ids=[str(s) for s in TILES])
+def test_dense_larger_tiles(i, dtype):
+    """Sizes that get the larger product tiles, with edges in every direction; rows at odd places for every other one."""
+    from smrt_amd.autoencode import dense, dense_backward, pack_rows, unpack_rows
+    m, k, n = TILES[i]
+    rng = np.random.default_rng(300 + i)
+    x, w, g = make(rng, dtype, m, k), make(rng, dtype, k, n, scale=k ** -0.5), make(rng, dtype, m, n)
+    put = odd_rows if i % 2 else (lambda v: v.cuda())
+    y = dense(put(x), put(w))
+    check_dense(x, w, None, None, "identity", y, None, dtype)
+    dx, dw, db = dense_backward(put(g), put(x), put(w))
+    check_dense_backward(g, x, w, None, "identity", dx, dw, db, dtype)
+    px = pack_rows(put(x))
+    _, dw, _ = dense_backward(put(g), px, put(w), need_x=False, need_bias=False)
+    check_dense_backward(g, unpack_rows(px).cpu(), w, None, "identity", None, dw, None, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_grouped_larger_tiles(dtype):
+    from smrt_amd.autoencode import dense_grouped, dense_grouped_backward
+    rng = np.random.default_rng(400)
+    ends, m, k, n = [9000, 9000, 21001, 40000], 40100, 130, 270
+    x, w, b, g = make(rng, dtype, m, k), make(rng, dtype, 4, k, n, scale=k ** -0.5), make(rng, dtype, 4, n), make(rng, dtype, m, n)
+    e = torch.tensor(ends, device="cuda")
+    y, saved = dense_grouped(x.cuda(), e, w.cuda(), b.cuda(), activation="sigmoid", save="activation")
+    dx, dw, db = dense_grouped_backward(g.cuda(), x.cuda(), e, w.cuda(), saved, activation="sigmoid")
+    lo = 0
+    for j, hi in enumerate(ends):
+        s, a = slice(lo, hi), saved[lo:hi].cpu()
+        check_dense(x[s], w[j], b[j], None, "sigmoid", y[s], saved[s], dtype)
+        check_dense_backward(g[s], x[s], w[j], a, "sigmoid", dx[s], dw[j], db[j], dtype)
+        lo = hi
+    assert not y[lo:].any() and not dx[lo:].any()

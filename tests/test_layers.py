@@ -92,7 +92,7 @@ def _dense_args(**kw):
 
 
 FORWARD_BAD = [dict(dtype=3), dict(dtype=-1), dict(activation=5), dict(rows=-1), dict(rows=1 << 31), dict(k=1 << 31), dict(groups=0),
-               dict(groups=2), dict(groups=1 << 16, ends=0x1000), dict(ldx=7), dict(ldw=15), dict(ldy=15), dict(lda=15), dict(x=0), dict(w=0), dict(y=0),
+               dict(groups=2), dict(groups=1 << 16, ends=0x1000), dict(ldx=7), dict(ldx=(1 << 21) + 1), dict(ldw=(1 << 21) + 1), dict(ldw=15), dict(ldy=15), dict(lda=15), dict(x=0), dict(w=0), dict(y=0),
                dict(x_scale=0x90000), dict(residual=0x100000, ldr=15), dict(groups=2, ends=0x1000, w_stride=64), dict(w_stride=-1),
                dict(groups=2, ends=0x1000, w_stride=128, bias=0x1000, bias_stride=15),
                dict(a_scale=0x90000, lda=16), dict(a_scale=0x90000, lda=32, ld_a_scale=0),
