@@ -21,11 +21,15 @@ constexpr int PACK_BLOCK = 32;            // columns of a row that share one sca
 // Rows move in pieces of 8 columns.  The tensors are a user's: rows may start at any element, so the pieces are read and
 // written as memory of the element's own alignment (global loads and stores take any address on gfx950; 16 bytes stay one
 // instruction).  A piece that the row's end cuts goes element by element.
-template <class T> struct alignas(sizeof(T)) Piece { T v[8]; };
+typedef uint32_t Words4 __attribute__((ext_vector_type(4), aligned(2), may_alias));
 
 template <class T> __device__ __forceinline__ void load8(const T* __restrict__ p, int valid, T (&v)[8]) {
     if (valid >= 8) {
-        __builtin_memcpy(v, p, 8 * sizeof(T));
+#pragma unroll
+        for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
+            const u32x4 w = ((const Words4*)p)[h];
+            __builtin_memcpy((char*)v + 16 * h, &w, 16);
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = j < valid ? p[j] : (T)0.0f;
@@ -33,7 +37,12 @@ template <class T> __device__ __forceinline__ void load8(const T* __restrict__ p
 }
 template <class T> __device__ __forceinline__ void store8(T* p, int valid, const T (&v)[8]) {
     if (valid >= 8) {
-        __builtin_memcpy(p, v, 8 * sizeof(T));
+#pragma unroll
+        for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
+            u32x4 w;
+            __builtin_memcpy(&w, (const char*)v + 16 * h, 16);
+            ((Words4*)p)[h] = w;
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) if (j < valid) p[j] = v[j];
@@ -146,44 +155,117 @@ __device__ __forceinline__ int clamp_end(const int64_t* __restrict__ ends, int g
     const int64_t e = ends[g];
     return e < 0 ? 0 : e > rows ? rows : (int)e;
 }
-// rows of group g
-__device__ __forceinline__ RowSpan group_rows(const int64_t* __restrict__ ends, int g, int rows) {
-    const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int i = lane; i < g; i += 64) { const int e = clamp_end(ends, i, g, rows); before = e > before ? e : before; }
+__device__ __forceinline__ int wave_max_scan(int v) {
 #pragma unroll
-    for (int d = 32; d; d >>= 1) { const int o = __shfl_xor(before, d); before = o > before ? o : before; }
-    const int e = clamp_end(ends, g, g + 1, rows);
-    return {g, before, e > before ? e : before};
+    for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(v, d); if ((int)(threadIdx.x & 63) >= d && o > v) v = o; }
+    return v;
+}
+__device__ __forceinline__ int wave_sum_scan(int v) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(v, d); if ((int)(threadIdx.x & 63) >= d) v += o; }
+    return v;
+}
+// Calls f(group, begin, end) for 64 groups at a time, a group a lane, in order, until f returns true.  Lanes behind the last group see an empty one.
+template <class F> __device__ __forceinline__ int walk_groups(const int64_t* __restrict__ ends, int n_groups, int rows, F f) {
+    int end0 = 0;
+    for (int base = 0; base < n_groups; base += 64) {
+        const int g = base + (int)(threadIdx.x & 63);
+        int e = wave_max_scan(clamp_end(ends, g, n_groups, rows));
+        e = e > end0 ? e : end0;
+        int begin = __shfl_up(e, 1);
+        if ((threadIdx.x & 63) == 0) begin = end0;
+        if (f(g, begin, e)) return end0;
+        end0 = __shfl(e, 63);
+    }
+    return end0;
 }
 // the t-th tile of `tile` rows, where no tile crosses from one group into the next; behind the last group come the rows
 // that no group has
 __device__ __forceinline__ RowSpan tile_rows(const int64_t* __restrict__ ends, int n_groups, int rows, int t, int tile) {
-    const int lane = threadIdx.x & 63;
-    int end0 = 0, tiles0 = 0;
-    for (int base = 0; base < n_groups; base += 64) {
-        int e = clamp_end(ends, base + lane, n_groups, rows);
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(e, d); if (lane >= d && o > e) e = o; }
-        e = e > end0 ? e : end0;
-        int prev = __shfl_up(e, 1);
-        if (lane == 0) prev = end0;
-        const int own = (e - prev + tile - 1) / tile;
-        int sum = own;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(sum, d); if (lane >= d) sum += o; }
-        sum += tiles0;
+    RowSpan s = {-1, 0, rows};
+    int tiles0 = 0;
+    const int last = walk_groups(ends, n_groups, rows, [&](int g, int begin, int end) {
+        const int own = (end - begin + tile - 1) / tile, sum = tiles0 + wave_sum_scan(own);
         const unsigned long long hit = __ballot(t < sum);
         if (hit) {
             const int f = __builtin_ctzll(hit);
-            const int first = __shfl(sum - own, f), begin = __shfl(prev, f), end = __shfl(e, f);
-            return {base + f, begin + (t - first) * tile, end};
+            s = {__shfl(g, f), __shfl(begin, f) + (t - __shfl(sum - own, f)) * tile, __shfl(end, f)};
         }
-        end0 = __shfl(e, 63);
         tiles0 = __shfl(sum, 63);
+        return hit != 0;
+    });
+    if (s.group < 0) {
+        const long r0 = (long)last + (long)(t - tiles0) * tile;
+        s.r0 = r0 < rows ? (int)r0 : rows;
     }
-    const long r0 = (long)end0 + (long)(t - tiles0) * tile;
-    return {-1, r0 < rows ? (int)r0 : rows, rows};
+    return s;
+}
+
+// how many tiles there are, the ones of rows that no group has among them
+__device__ __forceinline__ int count_tiles(const int64_t* __restrict__ ends, int n_groups, int rows, int tile) {
+    if (!ends) return (rows + tile - 1) / tile;
+    int n = 0;
+    const int last = walk_groups(ends, n_groups, rows, [&](int, int begin, int end) { n += (end - begin + tile - 1) / tile; return false; });
+#pragma unroll
+    for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
+    return n + (rows - last + tile - 1) / tile;
+}
+
+// ---- sums over a group's rows.  The rows are cut into chunks of `chunk`, none across groups, so that a large group does not
+// make one workgroup late.  A group of one chunk has its result written at once; the chunks of the larger groups are numbered one
+// after the other, each fills the slab of its number, and the join adds a group's slabs in their order.  A group
+// without rows has no chunk, and zeros from the join.  Larger groups have at most rows / chunk + min(groups, rows / chunk) chunks.
+struct Chunk { int group, r0, r1, slab; };       // slab -1: the group's only chunk; group -1: nothing
+struct Slabs { int first, count; };              // count 0: no rows, 1: written at once
+
+// chunk c: those of the larger groups first, then the groups of one chunk
+__device__ __forceinline__ Chunk chunk_rows(const int64_t* __restrict__ ends, int n_groups, int rows, int c, int chunk) {
+    Chunk r = {-1, 0, 0, -1};
+    if (!ends) {
+        const long r0 = (long)c * chunk;
+        if (r0 < rows) r = {0, (int)r0, rows - r0 > chunk ? (int)r0 + chunk : rows, rows > chunk ? c : -1};
+        return r;
+    }
+    int before = 0;
+#pragma unroll 1
+    for (int single = 0; single < 2 && r.group < 0; ++single)
+        walk_groups(ends, n_groups, rows, [&](int g, int begin, int end) {
+            const int n = end - begin, own = single ? (n > 0 && n <= chunk) : n > chunk ? (n - 1) / chunk + 1 : 0;
+            const int sum = before + wave_sum_scan(own);
+            const unsigned long long hit = __ballot(c < sum);
+            if (hit) {
+                const int f = __builtin_ctzll(hit);
+                const int r0 = __shfl(begin, f) + (c - __shfl(sum - own, f)) * chunk, r1 = __shfl(end, f);
+                r = {__shfl(g, f), r0, r1 - r0 > chunk ? r0 + chunk : r1, single ? -1 : c};
+            }
+            before = __shfl(sum, 63);
+            return hit != 0;
+        });
+    return r;
+}
+__device__ __forceinline__ int count_chunks(const int64_t* __restrict__ ends, int n_groups, int rows, int chunk) {
+    if (!ends) return (rows + chunk - 1) / chunk;
+    int n = 0;
+    walk_groups(ends, n_groups, rows, [&](int, int begin, int end) { n += (end - begin + chunk - 1) / chunk; return false; });
+#pragma unroll
+    for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
+    return n;
+}
+__device__ __forceinline__ Slabs group_slabs(const int64_t* __restrict__ ends, int n_groups, int rows, int group, int chunk) {
+    if (!ends) return {0, (rows + chunk - 1) / chunk};
+    Slabs s = {0, 0};
+    int before = 0;
+    walk_groups(ends, n_groups, rows, [&](int g, int begin, int end) {
+        const int n = end - begin, own = n > chunk ? (n - 1) / chunk + 1 : 0, sum = before + wave_sum_scan(own);
+        const unsigned long long hit = __ballot(g == group);
+        if (hit) {
+            const int f = __builtin_ctzll(hit), rows_f = __shfl(n, f);
+            s = {__shfl(sum - own, f), rows_f > chunk ? __shfl(own, f) : rows_f > 0};
+        }
+        before = __shfl(sum, 63);
+        return hit != 0;
+    });
+    return s;
 }
 
 }  // namespace layers

@@ -9,7 +9,7 @@ template <class T, int LAYOUT, bool PACKED, int BM, int BN, int BK, int WAVES_M,
 static hipError_t run(const GemmArgs& in, hipStream_t stream) {
     GemmArgs g = in;
     g.tiles_n = (g.N + BN - 1) / BN;
-    const int64_t tiles_m = LAYOUT == LAYOUT_DW ? (int64_t)((g.M + BM - 1) / BM) * g.groups * g.splits
+    const int64_t tiles_m = LAYOUT == LAYOUT_DW ? (int64_t)((g.M + BM - 1) / BM) * max_chunks(g.ends != nullptr, g.rows, g.chunk, g.groups)
                           : g.ends             ? (int64_t)g.rows / BM + g.groups + 1
                                                : (g.rows + BM - 1) / BM;
     const int64_t blocks = tiles_m * g.tiles_n;

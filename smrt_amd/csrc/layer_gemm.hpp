@@ -23,7 +23,7 @@ struct GemmArgs {
     const uint8_t* A_scale; int64_t lds_scale;     // x in its 8-bit form: A is int8, its scale bytes here
     const void* B; int64_t ldb, strideB;           // forward, dx: W [k][n] per group;  dW: dz [rows][n]
     void* C; int64_t ldc, strideC;                 // y, dx or dW (per group)
-    float* slab;                                   // dW with splits: [splits][groups][M][N] partial sums
+    float* slab;                                   // dW: [chunks of the larger groups][M][N] sums
     const void* bias; int64_t stride_bias;         // forward only, may be null
     const void* residual; int64_t ldr;             // forward only, may be null
     void* act_out; int64_t ld_act;                 // forward only, may be null: act(z) where it is not y
@@ -31,7 +31,7 @@ struct GemmArgs {
     const int64_t* ends; int32_t groups, keep_rest; // ends null: one group of all rows
     int32_t rows;                                  // of x
     int32_t M, N, K;                               // of the product (dW: M = k, N = n, K = rows)
-    int32_t splits;                                // dW: slices of a group's rows
+    int32_t chunk;                                 // dW: rows a workgroup sums over (chunk_rows)
     int32_t act;
     int32_t tiles_n;
 };
@@ -249,29 +249,25 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gem
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wk = wave / (WAVES_M * WAVES_N), wm = (wave / WAVES_N % WAVES_M) * WM, wn = (wave % WAVES_N) * WN;
 
-    // which tile, of which group
-    int bid = xcd_tile(blockIdx.x, gridDim.x);
+    // Which tile, of which group.  The grid is as large as any ends need; the workgroups too many are the last ones, so that every
+    // XCD has as much to do.
+    const int tiles_m = (g.M + BM - 1) / BM;
+    const int count = LAYOUT == LAYOUT_DW ? count_chunks(g.ends, g.groups, g.rows, g.chunk) * tiles_m : count_tiles(g.ends, g.groups, g.rows, BM);
+    const int total = __builtin_amdgcn_readfirstlane(count) * g.tiles_n;
+    if ((int)blockIdx.x >= total) return;
+    int bid = xcd_tile(blockIdx.x, total);
     const int tn = bid % g.tiles_n;
     bid /= g.tiles_n;
-    int m0, m_end, k0 = 0, k_end = g.K, group = 0, slice = 0;
+    int m0, m_end, k0 = 0, k_end = g.K, group = 0, slab = -1;
     if constexpr (LAYOUT == LAYOUT_DW) {
-        const int tiles_m = (g.M + BM - 1) / BM;
         m0 = (bid % tiles_m) * BM;
         m_end = g.M;
-        bid /= tiles_m;
-        group = bid % g.groups;
-        slice = bid / g.groups;
-        int r0 = 0, r1 = g.rows;
-        if (g.ends) {
-            const RowSpan s = group_rows(g.ends, group, g.rows);
-            r0 = __builtin_amdgcn_readfirstlane(s.r0);
-            r1 = __builtin_amdgcn_readfirstlane(s.r1);
-        }
-        int per = (r1 - r0 + g.splits - 1) / g.splits;
-        per = (per + BK - 1) / BK * BK;
-        const long b0 = r0 + (long)slice * per;
-        k0 = b0 < r1 ? (int)b0 : r1;
-        k_end = r1 - k0 > per ? k0 + per : r1;
+        const Chunk c = chunk_rows(g.ends, g.groups, g.rows, bid / tiles_m, g.chunk);
+        group = __builtin_amdgcn_readfirstlane(c.group);
+        if (group < 0) return;
+        k0 = __builtin_amdgcn_readfirstlane(c.r0);
+        k_end = __builtin_amdgcn_readfirstlane(c.r1);
+        slab = __builtin_amdgcn_readfirstlane(c.slab);
     } else {
         if (g.ends) {
             const RowSpan s = tile_rows(g.ends, g.groups, g.rows, bid, BM);
@@ -472,8 +468,8 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gem
             const int row = row0 + it * ROWS_PER, valid = row < m_end ? cvalid : 0;
             if constexpr (LAYOUT == LAYOUT_DW) {
                 if (valid <= 0) continue;
-                if (g.slab) store8(g.slab + (((int64_t)slice * g.groups + group) * g.M + row) * g.N + col, valid, v[it]);
-                else        store8f((T*)g.C + (int64_t)group * g.strideC + (int64_t)row * g.ldc + col, valid, v[it]);
+                if (slab >= 0) store8(g.slab + ((int64_t)slab * g.M + row) * g.N + col, valid, v[it]);
+                else           store8f((T*)g.C + (int64_t)group * g.strideC + (int64_t)row * g.ldc + col, valid, v[it]);
             } else if constexpr (LAYOUT == LAYOUT_DX) {
                 if (valid > 0 && !(rest && g.keep_rest)) store8f((T*)g.C + (int64_t)row * g.ldc + col, valid, v[it]);
             } else {

@@ -16,47 +16,56 @@ constexpr int MAX_GROUPS = 65535;
 
 // ------------------------------------------------------------------------------------------------ dz = g * act'(a), column sums
 // One pass over g (and a): writes dz for the two products that read it, and sums its columns into db on the way (in fp32, from
-// the values before they are rounded to T).  256 columns x 8 rows per workgroup step; a workgroup owns a slice of one group's rows.
+// the values before they are rounded to T).  A workgroup has 256 columns of a chunk of DZ_CHUNK rows (chunk_rows), 8 rows x 4 at a time.
+constexpr int DZ_CHUNK = 64;
 struct DzArgs {
     const void* grad; int64_t ldg;
     const void* a; int64_t lda; const uint8_t* a_scale; int64_t ld_a_scale;
     void* dz; int64_t ld_dz;                       // null: the identity, whose dz is g
-    float* part;                                   // [slices][groups][n], or null where slices == 1
+    float* part;                                   // [chunks of the larger groups][n]
     void* db; int64_t db_stride;                   // null: not wanted
-    const int64_t* ends; int32_t groups, rows, n, slices, act, col_blocks;
+    const int64_t* ends; int32_t groups, rows, n, act, col_blocks;
 };
 
 template <class T, bool PACKED> __global__ void __launch_bounds__(256) dz_kernel(DzArgs p) {
     __shared__ float sums[8][256];
-    int bid = blockIdx.x;
-    const int cb = bid % p.col_blocks;
-    bid /= p.col_blocks;
-    const int group = bid % p.groups, slice = bid / p.groups;
-    int r0 = 0, r1 = p.rows;
-    if (p.ends) { const RowSpan s = group_rows(p.ends, group, p.rows); r0 = s.r0; r1 = s.r1; }
-    const int per = (r1 - r0 + p.slices - 1) / p.slices;
-    const long first = r0 + (long)slice * per;
-    const int lo = first < r1 ? (int)first : r1, hi = r1 - lo > per ? lo + per : r1;
+    const int cb = blockIdx.x % p.col_blocks;
+    const Chunk chunk = chunk_rows(p.ends, p.groups, p.rows, blockIdx.x / p.col_blocks, DZ_CHUNK);
+    if (chunk.group < 0) return;
+    const int lo = chunk.r0, hi = chunk.r1;
     const int col = cb * 256 + (threadIdx.x & 31) * 8, valid = p.n - col;
     float sum[8] = {};
     if (valid > 0) {
-        for (int row = lo + (threadIdx.x >> 5); row < hi; row += 8) {
-            float g[8];
-            load8f((const T*)p.grad + (int64_t)row * p.ldg + col, valid, g);
-            if (p.dz) {
-                float a[8];
+        constexpr int U = 4;                       // rows in flight a thread: a row's pieces are a round trip to memory
+        for (int row = lo + (threadIdx.x >> 5); row < hi; row += 8 * U) {
+            float g[U][8], a[U][8];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = row + 8 * u, has = r < hi ? valid : 0;
+                load8f((const T*)p.grad + (int64_t)r * p.ldg + col, has, g[u]);
+                if (!p.dz) continue;
                 if constexpr (PACKED) {
-                    u32x2 q;
-                    __builtin_memcpy(&q, (const int8_t*)p.a + (int64_t)row * p.lda + col, 8);
-                    unpack8(q, unpack_scale(p.a_scale[(int64_t)row * p.ld_a_scale + col / PACK_BLOCK]), a);
+                    u32x2 q = {0u, 0u};
+                    int byte = 0;
+                    if (has > 0) {
+                        __builtin_memcpy(&q, (const int8_t*)p.a + (int64_t)r * p.lda + col, 8);
+                        byte = p.a_scale[(int64_t)r * p.ld_a_scale + col / PACK_BLOCK];
+                    }
+                    unpack8(q, unpack_scale(byte), a[u]);
                 } else {
-                    load8f((const T*)p.a + (int64_t)row * p.lda + col, valid, a);
+                    load8f((const T*)p.a + (int64_t)r * p.lda + col, has, a[u]);
                 }
-                layer_act_grad8(p.act, a, g);
-                store8f((T*)p.dz + (int64_t)row * p.ld_dz + col, valid, g);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum[j] += g[j];
+            for (int u = 0; u < U; ++u) {
+                const int r = row + 8 * u;
+                if (p.dz) {
+                    layer_act_grad8(p.act, a[u], g[u]);
+                    if (r < hi) store8f((T*)p.dz + (int64_t)r * p.ld_dz + col, valid, g[u]);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[j] += g[u][j];
+            }
         }
     }
     if (!p.db) return;
@@ -68,32 +77,35 @@ template <class T, bool PACKED> __global__ void __launch_bounds__(256) dz_kernel
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) s += sums[i][threadIdx.x];
-        if (p.part) p.part[((int64_t)slice * p.groups + group) * p.n + c] = s;
-        else ((T*)p.db)[(int64_t)group * p.db_stride + c] = (T)s;
+        if (chunk.slab >= 0) p.part[(int64_t)chunk.slab * p.n + c] = s;
+        else ((T*)p.db)[(int64_t)chunk.group * p.db_stride + c] = (T)s;
     }
 }
 
 // ------------------------------------------------------------------------------------------------ joining of partial sums
-// out[row][col] = sum over slabs of slab[s][row][col], in the order of s: the result does not depend on timing.
-struct JoinPart {                     // blocks == 0: nothing
-    const float* slab; int64_t slabs, rows, cols, slab_stride;     // slab s at s * slab_stride
-    void* out; int64_t ld, group_rows, group_stride;               // row r of out: (r / group_rows) * group_stride + (r % group_rows) * ld
-    int32_t out_f32;
-    int32_t blocks;
+// out[group][row][col] = sum over the group's slabs (group_slabs), in their order: the result does not depend on timing.
+// A group of one chunk has its result already, one without rows gets zeros.
+struct JoinPart {
+    const float* slab; int64_t slab_stride;          // slab s at s * slab_stride: [out_rows][cols]
+    const int64_t* ends; int32_t groups, rows, chunk;
+    int32_t out_rows, cols; void* out; int64_t ld, group_stride;
+    int32_t out_f32, group_blocks, blocks;           // workgroups a group and altogether; 0: nothing to join
 };
-// SL threads share the slabs of a piece of 8 columns: many for the long sums over workgroups, one for the few splits of a product
+// SL threads share the slabs of a piece of 8 columns: many for the long sums over workgroups, one for the few chunks of a product
 template <class T, int SL> __device__ __forceinline__ void join(const JoinPart& p, int block, float (*lds)[8]) {
     constexpr int PIECES = 256 / SL;
-    const int64_t per_row = (p.cols + 7) / 8;
+    const int group = block / p.group_blocks;
+    const Slabs slabs = group_slabs(p.ends, p.groups, p.rows, group, p.chunk);
+    if (slabs.count == 1) return;
+    const uint32_t per_row = (uint32_t)(p.cols + 7) / 8;
     const int sl = threadIdx.x / PIECES;
-    const int64_t piece = (int64_t)block * PIECES + threadIdx.x % PIECES;
-    const int64_t row = piece / per_row, col = (piece % per_row) * 8;
-    const int valid = row < p.rows ? (int)(p.cols - col < 8 ? p.cols - col : 8) : 0;
+    const uint32_t piece = (uint32_t)(block - group * p.group_blocks) * PIECES + threadIdx.x % PIECES, row = piece / per_row;
+    const int col = (int)(piece - row * per_row) * 8, valid = row < (uint32_t)p.out_rows ? p.cols - col : 0;
     float sum[8] = {};
     if (valid > 0) {
-        const float* src = p.slab + row * p.cols + col;
+        const float* src = p.slab + slabs.first * p.slab_stride + (int64_t)row * p.cols + col;
 #pragma unroll 4
-        for (int64_t s = sl; s < p.slabs; s += SL) {
+        for (int s = sl; s < slabs.count; s += SL) {
             float v[8];
             load8f(src + s * p.slab_stride, valid, v);
 #pragma unroll
@@ -110,7 +122,7 @@ template <class T, int SL> __device__ __forceinline__ void join(const JoinPart& 
             for (int j = 0; j < 8; ++j) sum[j] += lds[i * PIECES + threadIdx.x][j];
     }
     if (valid <= 0) return;
-    const int64_t at = (row / p.group_rows) * p.group_stride + (row % p.group_rows) * p.ld + col;
+    const int64_t at = (int64_t)group * p.group_stride + (int64_t)row * p.ld + col;
     if (p.out_f32) store8((float*)p.out + at, valid, sum);
     else store8f((T*)p.out + at, valid, sum);
 }
@@ -119,10 +131,13 @@ template <class T, int SL0, int SL1> __global__ void __launch_bounds__(256) join
     if ((int)blockIdx.x < a.blocks) join<T, SL0>(a, blockIdx.x, lds);
     else join<T, SL1>(b, blockIdx.x - a.blocks, lds);
 }
-JoinPart join_part(const float* slab, int64_t slabs, int64_t slab_stride, int64_t rows, int64_t cols, void* out, int64_t ld, int64_t group_rows, int64_t group_stride,
-                   bool out_f32, int sl) {
-    const int64_t pieces = rows * ((cols + 7) / 8), per = 256 / sl;
-    return {slab, slabs, rows, cols, slab_stride, out, ld, std::max<int64_t>(group_rows, 1), group_stride, out_f32, (int32_t)((pieces + per - 1) / per)};
+// fills in group_blocks and blocks; false where that is more than a launch takes
+bool join_blocks(JoinPart& p, int sl) {
+    const int64_t pieces = (int64_t)p.out_rows * ((p.cols + 7) / 8), per = 256 / sl, blocks = (pieces + per - 1) / per;
+    if (pieces > 0x7fffffff || blocks * p.groups > 0x3fffffff) return false;
+    p.group_blocks = (int32_t)blocks;
+    p.blocks = (int32_t)blocks * p.groups;
+    return true;
 }
 
 // ------------------------------------------------------------------------------------------------ layer norm
@@ -293,26 +308,27 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_backward_kernel(No
 // ------------------------------------------------------------------------------------------------ the 8-bit form on its own
 struct PackArgs { const void* x; int64_t ldx; int8_t* q; int64_t ldq; uint8_t* scale; int64_t ld_scale; int64_t rows; int32_t n; void* out; };
 
-template <class T> __global__ void __launch_bounds__(256) pack_kernel(PackArgs p) {
-    const int64_t per_row = (int64_t)((p.n + PACK_BLOCK - 1) / PACK_BLOCK) * 4, total = p.rows * per_row;       // whole blocks: four lanes
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {      // stay together
-        const int64_t row = i / per_row;
-        const int col = (int)(i % per_row) * 8;
+// I: an index type that holds the number of pieces (a 64-bit division costs more than the rest of a piece)
+template <class T, class I> __global__ void __launch_bounds__(256) pack_kernel(PackArgs p) {
+    const I per_row = (I)((p.n + PACK_BLOCK - 1) / PACK_BLOCK) * 4, total = (I)p.rows * per_row;       // whole blocks: four lanes
+    for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < total; i += (I)gridDim.x * 256) {                // stay together
+        const I row = i / per_row;
+        const int col = (int)(i - row * per_row) * 8;
         float f[8];
-        load8f((const T*)p.x + row * p.ldx + col, p.n - col, f);
-        pack_block<T>(f, (int)(i & 3), true, p.q + row * p.ldq + col, p.scale + row * p.ld_scale + col / PACK_BLOCK);
+        load8f((const T*)p.x + (int64_t)row * p.ldx + col, p.n - col, f);
+        pack_block<T>(f, (int)(i & 3), true, p.q + (int64_t)row * p.ldq + col, p.scale + (int64_t)row * p.ld_scale + col / PACK_BLOCK);
     }
 }
-template <class T> __global__ void __launch_bounds__(256) unpack_kernel(PackArgs p) {
-    const int64_t per_row = (p.n + 7) / 8, total = p.rows * per_row;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / per_row;
-        const int col = (int)(i % per_row) * 8;
+template <class T, class I> __global__ void __launch_bounds__(256) unpack_kernel(PackArgs p) {
+    const I per_row = (I)((p.n + 7) / 8), total = (I)p.rows * per_row;
+    for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < total; i += (I)gridDim.x * 256) {
+        const I row = i / per_row;
+        const int col = (int)(i - row * per_row) * 8;
         u32x2 q;
-        __builtin_memcpy(&q, p.q + row * p.ldq + col, 8);
+        __builtin_memcpy(&q, p.q + (int64_t)row * p.ldq + col, 8);
         float f[8];
-        unpack8(q, unpack_scale(p.scale[row * p.ld_scale + col / PACK_BLOCK]), f);
-        store8f((T*)p.out + row * p.ldx + col, p.n - col, f);
+        unpack8(q, unpack_scale(p.scale[(int64_t)row * p.ld_scale + col / PACK_BLOCK]), f);
+        store8f((T*)p.out + (int64_t)row * p.ldx + col, p.n - col, f);
     }
 }
 
@@ -351,7 +367,6 @@ hipError_t gemm(int dtype, int layout, const GemmPlan& p, const GemmArgs& g, hip
 
 struct BackwardPlan {
     bool need_dz, need_sum;
-    int dz_slices;
     GemmPlan dw;
     int64_t ld_dz, dz_bytes, slab_off, slab_bytes, part_off, part_bytes, total;
 };
@@ -362,12 +377,9 @@ BackwardPlan plan_backward(const smrt_dense* p) {
     b.need_sum = p->db != nullptr;
     b.ld_dz = pad(p->n, 8);
     b.dz_bytes = b.need_dz ? pad(p->rows * b.ld_dz * es, 256) : 0;
-    const int64_t col_blocks = (p->n + 255) / 256, avg = p->rows / G;
-    // slices of a group's rows: enough workgroups for every CU several times over, none with fewer than 64 rows
-    b.dz_slices = (int)std::max<int64_t>(1, std::min<int64_t>(avg / 64, 2048 / std::max<int64_t>(1, col_blocks * G)));
-    b.part_bytes = b.need_sum && b.dz_slices > 1 ? pad((int64_t)b.dz_slices * G * p->n * 4, 256) : 0;
+    b.part_bytes = b.need_sum ? pad(max_slabs(p->rows, DZ_CHUNK, G) * p->n * 4, 256) : 0;
     b.dw = plan_gemm(LAYOUT_DW, p->dtype == SMRT_F32, p->rows, p->k, p->n, G);
-    b.slab_bytes = p->dw && b.dw.splits > 1 ? pad((int64_t)b.dw.splits * G * p->k * p->n * 4, 256) : 0;
+    b.slab_bytes = p->dw ? pad(max_slabs(p->rows, b.dw.chunk, G) * p->k * p->n * 4, 256) : 0;
     b.slab_off = b.dz_bytes;
     b.part_off = b.slab_off + b.slab_bytes;
     b.total = b.part_off + b.part_bytes;
@@ -379,9 +391,11 @@ template <class F> hipError_t by_type(int dtype, F f) {
 }
 
 template <class T> hipError_t launch_dz(const DzArgs& d, hipStream_t s) {
-    const unsigned blocks = (unsigned)((int64_t)d.col_blocks * d.groups * d.slices);
-    if (d.a_scale) hipLaunchKernelGGL((dz_kernel<T, true>), dim3(blocks), dim3(256), 0, s, d);
-    else hipLaunchKernelGGL((dz_kernel<T, false>), dim3(blocks), dim3(256), 0, s, d);
+    const int64_t blocks = (int64_t)d.col_blocks * max_chunks(d.ends != nullptr, d.rows, DZ_CHUNK, d.groups);
+    if (blocks == 0) return hipSuccess;
+    if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+    if (d.a_scale) hipLaunchKernelGGL((dz_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, s, d);
+    else hipLaunchKernelGGL((dz_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, s, d);
     return hipGetLastError();
 }
 
@@ -401,7 +415,12 @@ template <class F> hipError_t by_width(int64_t n, F f) {
     return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
 }
 int norm_rows_per_block(int64_t n) { return n <= 64 ? 32 : n <= 128 ? 16 : n <= 256 ? 8 : n <= 1024 ? 4 : 1; }
-int norm_backward_blocks(int64_t rows, int64_t n) { return norm_blocks(rows, norm_rows_per_block(n), 512); }
+// 1024 workgroups keep enough rows in flight (512: 121 us at 65536 x 1024 bf16); up to four turns of one workgroup are over sooner
+// than the launch that would join two workgroups' sums
+int norm_backward_blocks(int64_t rows, int64_t n) {
+    const int per = norm_rows_per_block(n);
+    return rows <= 4 * per ? 1 : norm_blocks(rows, per, 1024);
+}
 
 int check_norm(const smrt_layer_norm* p, const char* who) {
     if (!p) return fail(who, "null argument");
@@ -429,6 +448,7 @@ int check_pack(const char* who, int dtype, const void* x, int64_t ldx, int64_t r
     if (rows && n && (!x || !q || !scale)) return fail(who, "null pointer");
     return 0;
 }
+constexpr int64_t SMALL_INDEX = 0xffffffffll - 256 * 256 * 64;       // an index and the grid's stride stay below 2^32
 unsigned grid_of(int64_t items) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((items + 255) / 256, 256 * 32)); }
 
 }  // namespace
@@ -457,7 +477,7 @@ extern "C" int smrt_dense_forward(const smrt_dense* p, void* hip_stream) {
     if (p->a && p->a_scale) { g.q_out = (int8_t*)p->a; g.ldq = p->lda; g.q_scale = p->a_scale; g.ldq_scale = p->ld_a_scale; }
     else if (p->a) { g.act_out = p->a; g.ld_act = p->lda; }
     g.ends = p->ends; g.groups = p->groups; g.keep_rest = p->keep_rest; g.rows = (int32_t)p->rows;
-    g.M = (int32_t)p->rows; g.N = (int32_t)p->n; g.K = (int32_t)p->k; g.splits = 1; g.act = p->activation;
+    g.M = (int32_t)p->rows; g.N = (int32_t)p->n; g.K = (int32_t)p->k; g.act = p->activation;
     return launched(who, gemm(p->dtype, LAYOUT_FORWARD, plan_gemm(LAYOUT_FORWARD, p->dtype == SMRT_F32, p->rows, p->rows, p->n, p->groups), g, (hipStream_t)hip_stream));
 }
 
@@ -486,19 +506,18 @@ extern "C" int smrt_dense_backward(const smrt_dense* p, void* workspace, int64_t
     char* const ws = (char*)workspace;
     const void* dz = p->grad;
     int64_t ld_dz = p->ldg;
-    float* const part = b.part_bytes ? (float*)(ws + b.part_off) : nullptr;
     if (p->n && (b.need_dz || b.need_sum)) {
         DzArgs d = {};
         d.grad = p->grad; d.ldg = p->ldg; d.a = p->a; d.lda = p->lda;
         d.a_scale = b.need_dz ? p->a_scale : nullptr; d.ld_a_scale = p->ld_a_scale;
         if (b.need_dz) { d.dz = ws; d.ld_dz = b.ld_dz; dz = ws; ld_dz = b.ld_dz; }
-        d.part = part; d.db = p->db; d.db_stride = p->bias_stride;
-        d.ends = p->ends; d.groups = p->groups; d.rows = (int32_t)p->rows; d.n = (int32_t)p->n; d.slices = b.dz_slices; d.act = p->activation;
+        d.part = (float*)(ws + b.part_off); d.db = p->db; d.db_stride = p->bias_stride;
+        d.ends = p->ends; d.groups = p->groups; d.rows = (int32_t)p->rows; d.n = (int32_t)p->n; d.act = p->activation;
         d.col_blocks = (int32_t)((p->n + 255) / 256);
         if (hipError_t e = by_type(p->dtype, [&](auto t) { return launch_dz<decltype(t)>(d, stream); }); e != hipSuccess) return launched(who, e);
     }
     GemmArgs g = {};
-    g.ends = p->ends; g.groups = p->groups; g.keep_rest = p->keep_rest; g.rows = (int32_t)p->rows; g.splits = 1;
+    g.ends = p->ends; g.groups = p->groups; g.keep_rest = p->keep_rest; g.rows = (int32_t)p->rows;
     if (p->dx && p->rows && p->k) {
         g.A = dz; g.lda = ld_dz; g.B = p->w; g.ldb = p->ldw; g.strideB = p->w_stride; g.C = p->dx; g.ldc = p->lddx;
         g.M = (int32_t)p->rows; g.N = (int32_t)p->k; g.K = (int32_t)p->n;
@@ -507,23 +526,26 @@ extern "C" int smrt_dense_backward(const smrt_dense* p, void* workspace, int64_t
     const bool dw = p->dw && p->k && p->n;
     if (dw) {
         g.A = p->x; g.lda = p->ldx; g.A_scale = p->x_scale; g.lds_scale = p->ld_x_scale; g.B = dz; g.ldb = ld_dz; g.strideB = 0;
-        g.C = p->dw; g.ldc = p->lddw; g.strideC = p->dw_stride; g.slab = b.slab_bytes ? (float*)(ws + b.slab_off) : nullptr;
-        g.M = (int32_t)p->k; g.N = (int32_t)p->n; g.K = (int32_t)p->rows; g.splits = b.dw.splits;
+        g.C = p->dw; g.ldc = p->lddw; g.strideC = p->dw_stride; g.slab = (float*)(ws + b.slab_off);
+        g.M = (int32_t)p->k; g.N = (int32_t)p->n; g.K = (int32_t)p->rows; g.chunk = b.dw.chunk;
         if (hipError_t e = gemm(p->dtype, LAYOUT_DW, b.dw, g, stream); e != hipSuccess) return launched(who, e);
     }
-    if ((dw && b.slab_bytes) || part) {
-        JoinPart jw = {}, jb = {};
-        if (dw && b.slab_bytes) jw = join_part((const float*)(ws + b.slab_off), b.dw.splits, p->groups * p->k * p->n, p->groups * p->k, p->n, p->dw, p->lddw, p->k, p->dw_stride, false, 1);
-        if (part && p->n) jb = join_part(part, b.dz_slices, p->groups * p->n, p->groups, p->n, p->db, 0, 1, p->bias_stride, false, 32);
-        if (jw.blocks + jb.blocks) {
-            const hipError_t e = by_type(p->dtype, [&](auto t) {
-                hipLaunchKernelGGL((join_kernel<decltype(t), 1, 32>), dim3(jw.blocks + jb.blocks), dim3(256), 0, stream, jw, jb);
-                return hipGetLastError();
-            });
-            if (e != hipSuccess) return launched(who, e);
-        }
+    // one group with exactly one chunk has nothing to join; groups may be empty or larger
+    JoinPart jw = {}, jb = {};
+    if (dw && !(p->groups == 1 && !p->ends && p->rows > 0 && p->rows <= b.dw.chunk)) {
+        jw = {(const float*)(ws + b.slab_off), p->k * p->n, p->ends, p->groups, (int32_t)p->rows, b.dw.chunk, (int32_t)p->k, (int32_t)p->n, p->dw, p->lddw,
+              p->dw_stride, false};
+        if (!join_blocks(jw, 1)) return fail(who, "the weight gradient is too large");
     }
-    return 0;
+    if (p->db && p->n && !(p->groups == 1 && !p->ends && p->rows > 0 && p->rows <= DZ_CHUNK)) {
+        jb = {(const float*)(ws + b.part_off), p->n, p->ends, p->groups, (int32_t)p->rows, DZ_CHUNK, 1, (int32_t)p->n, p->db, 0, p->bias_stride, false};
+        if (!join_blocks(jb, 32)) return fail(who, "the bias gradient is too large");
+    }
+    if (jw.blocks + jb.blocks == 0) return 0;
+    return launched(who, by_type(p->dtype, [&](auto t) {
+        hipLaunchKernelGGL((join_kernel<decltype(t), 1, 32>), dim3(jw.blocks + jb.blocks), dim3(256), 0, stream, jw, jb);
+        return hipGetLastError();
+    }));
 }
 
 extern "C" int smrt_layer_norm_forward(const smrt_layer_norm* p, void* hip_stream) {
@@ -578,9 +600,9 @@ extern "C" int smrt_layer_norm_backward(const smrt_layer_norm* p, void* workspac
     if (e == hipSuccess && a.part) {
         // slabs of 2 n: the weight's half, then the bias's
         JoinPart jw = {}, jb = {};
-        const bool f32 = a.w_f32;
-        if (p->dw) jw = join_part(a.part, blocks, 2 * p->n, 1, p->n, p->dw, 0, 1, 0, f32, 32);
-        if (p->db) jb = join_part(a.part + p->n, blocks, 2 * p->n, 1, p->n, p->db, 0, 1, 0, f32, 32);
+        const int32_t n = (int32_t)p->n;
+        if (p->dw) { jw = {a.part, 2 * p->n, nullptr, 1, blocks, 1, 1, n, p->dw, 0, 0, a.w_f32}; join_blocks(jw, 32); }
+        if (p->db) { jb = {a.part + n, 2 * p->n, nullptr, 1, blocks, 1, 1, n, p->db, 0, 0, a.w_f32}; join_blocks(jb, 32); }
         e = by_type(p->dtype, [&](auto t) {
             hipLaunchKernelGGL((join_kernel<decltype(t), 32, 32>), dim3(jw.blocks + jb.blocks), dim3(256), 0, stream, jw, jb);
             return hipGetLastError();
@@ -596,7 +618,9 @@ extern "C" int smrt_pack_rows(int32_t dtype, const void* x, int64_t ldx, int64_t
     if (rows == 0 || n == 0) return 0;
     const PackArgs a = {x, ldx, q, ldq, scale, ld_scale, rows, (int32_t)n, nullptr};
     return launched(who, by_type(dtype, [&](auto t) {
-        hipLaunchKernelGGL((pack_kernel<decltype(t)>), dim3(grid_of(rows * (pad(n, PACK_BLOCK) / 8))), dim3(256), 0, (hipStream_t)hip_stream, a);
+        const int64_t pieces = rows * (pad(n, PACK_BLOCK) / 8);
+        if (pieces < SMALL_INDEX) hipLaunchKernelGGL((pack_kernel<decltype(t), uint32_t>), dim3(grid_of(pieces)), dim3(256), 0, (hipStream_t)hip_stream, a);
+        else hipLaunchKernelGGL((pack_kernel<decltype(t), uint64_t>), dim3(grid_of(pieces)), dim3(256), 0, (hipStream_t)hip_stream, a);
         return hipGetLastError();
     }));
 }
@@ -608,7 +632,9 @@ extern "C" int smrt_unpack_rows(int32_t dtype, const int8_t* q, int64_t ldq, con
     if (rows == 0 || n == 0) return 0;
     const PackArgs a = {nullptr, ldx, (int8_t*)q, ldq, (uint8_t*)scale, ld_scale, rows, (int32_t)n, x};
     return launched(who, by_type(dtype, [&](auto t) {
-        hipLaunchKernelGGL((unpack_kernel<decltype(t)>), dim3(grid_of(rows * ((n + 7) / 8))), dim3(256), 0, (hipStream_t)hip_stream, a);
+        const int64_t pieces = rows * ((n + 7) / 8);
+        if (pieces < SMALL_INDEX) hipLaunchKernelGGL((unpack_kernel<decltype(t), uint32_t>), dim3(grid_of(pieces)), dim3(256), 0, (hipStream_t)hip_stream, a);
+        else hipLaunchKernelGGL((unpack_kernel<decltype(t), uint64_t>), dim3(grid_of(pieces)), dim3(256), 0, (hipStream_t)hip_stream, a);
         return hipGetLastError();
     }));
 }

@@ -1,13 +1,18 @@
 // The layer products' launchers, one per element type (layer_gemm.hip), and which tile shape a product gets.
 #pragma once
 #include <algorithm>
+#include <cmath>
 #include "layer_gemm.hpp"
 
 namespace smrt {
 namespace layers {
 
+// chunks of groups larger than one (layer_common.hpp); with the groups of one chunk that many workgroups more
+inline int64_t max_slabs(int64_t rows, int64_t chunk, int64_t groups) { return groups == 1 ? (rows > chunk ? (rows + chunk - 1) / chunk : 0) : rows / chunk + std::min(groups, rows / chunk); }
+inline int64_t max_chunks(bool ends, int64_t rows, int64_t chunk, int64_t groups) { return ends ? max_slabs(rows, chunk, groups) + groups : (rows + chunk - 1) / chunk; }
+
 enum Tile : int { TILE_LARGE = 0, TILE_MEDIUM = 1, TILE_SMALL = 2 };
-struct GemmPlan { int tile, splits; };
+struct GemmPlan { int tile, chunk; };      // chunk: dW's rows a workgroup
 
 // 16-bit types have 256x256 (8 waves, one workgroup a CU), 128x128 (4 waves, two a CU) and 64x64 tiles whose 4 waves split the
 // summed index; fp32, whose three parts fill the registers sooner, the last two.  A launch takes its share of rounds over the 256 CUs, and at
@@ -18,21 +23,22 @@ struct GemmPlan { int tile, splits; };
 inline GemmPlan plan_gemm(int layout, bool f32, int64_t rows, int64_t m, int64_t n, int64_t groups) {
     constexpr int side[3] = {256, 128, 64};
     constexpr double chain[2][3] = {{30, 18.5, 10.5}, {1e9, 54, 24}}, round[2][3] = {{40, 11.7, 5.6}, {1e9, 48, 16}};
-    GemmPlan best = {TILE_SMALL, 1};
+    GemmPlan best = {TILE_SMALL, 512};
     double best_us = 1e30;
     for (int t = f32 ? 1 : 0; t < 3; ++t) {
         const int64_t tn = (n + side[t] - 1) / side[t];
-        GemmPlan p = {t, 1};
+        GemmPlan p = {t, 0};
         double us;
         if (layout == LAYOUT_DW) {
-            // the weight gradient sums over the rows: few tiles, so a group's rows go to `splits` workgroups a tile, whose sums are
-            // joined afterwards (the slabs pass through memory twice)
-            const int64_t tiles = (m + side[t] - 1) / side[t] * tn * groups, avg = std::max<int64_t>(rows / groups, 1);
-            const int64_t want = (t == TILE_LARGE ? 256 : 512) / std::max<int64_t>(tiles, 1);
-            p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(avg / 512, want));
-            const double part = (double)avg / p.splits / 1024.0;
-            us = part * std::max(chain[f32][t], round[f32][t] * (double)((tiles * p.splits + 255) / 256));
-            if (p.splits > 1) us += 2.0 * p.splits * groups * m * n * 4.0 / 5e6;
+            // the weight gradient sums over the rows: few tiles, so the rows are cut into chunks, a workgroup a tile and chunk, whose
+            // sums are joined afterwards (the slabs pass through memory twice); 512 rows at least, so that a chunk outweighs its slab
+            const int64_t tiles = (m + side[t] - 1) / side[t] * tn, want = std::max<int64_t>((t == TILE_LARGE ? 256 : 512) / std::max<int64_t>(tiles, 1), 1);
+            const int64_t chunk = std::max<int64_t>(512, (rows + want - 1) / want + 127) / 128 * 128;
+            p.chunk = (int)std::min<int64_t>(chunk, 1 << 30);
+            const double chunks = groups == 1 ? (double)((rows + chunk - 1) / chunk) : (double)rows / chunk + 0.5 * groups;
+            const double part = std::min((double)chunk, std::max(1.0, (double)rows / groups)) / 1024.0;
+            us = part * std::max(chain[f32][t], round[f32][t] * std::ceil(tiles * chunks / 256.0));
+            us += 2.0 * (double)max_slabs(rows, chunk, groups) * m * n * 4.0 / 5e6;
         } else {
             const int64_t tiles = (groups == 1 ? (rows + side[t] - 1) / side[t] : rows / side[t] + groups / 2) * tn;     // about half a tile a group is empty
             us = std::max(chain[f32][t], round[f32][t] * (double)((tiles + 255) / 256));
