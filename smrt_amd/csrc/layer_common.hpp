@@ -63,7 +63,31 @@ template <class T> __device__ __forceinline__ void store8f(T* p, int valid, cons
 
 // Activations.  Unlike act_fwd these hand a NaN on (relu of the training kernels is fmaxf, which drops it: there the loss
 // reports it; here the value is the user's).
-template <int N> __device__ __forceinline__ void layer_act(int act, float* v) {
+// e^v - 1 for v <= 0 in a dozen instructions (the library's takes several times that, which no memory traffic hides in a
+// product's epilogue): near 0, where the difference would cancel, the exponential's series, elsewhere the exponential itself, whose
+// error stays within a few units of 2^-24.  For fp32 the series goes to v^7 (next term below 2^-28 of v at 0.3); a result that is
+// rounded to 16 bits needs it to v^3 only (next term below 2^-19 of v at 0.03, the difference's error 2^-18 of it).
+template <class T> __device__ __forceinline__ float fast_expm1(float v) {
+    const float e = __builtin_amdgcn_exp2f(1.4426950408889634f * v) - 1.0f;
+    if constexpr (sizeof(T) == 2) {
+        const float s = fmaf(v, 1.0f / 6.0f, 0.5f);
+        return v > -0.03f ? fmaf(s * v, v, v) : e;
+    } else {
+        float s = fmaf(v, 1.0f / 5040.0f, 1.0f / 720.0f);
+        s = fmaf(s, v, 1.0f / 120.0f);
+        s = fmaf(s, v, 1.0f / 24.0f);
+        s = fmaf(s, v, 1.0f / 6.0f);
+        s = fmaf(s, v, 0.5f);
+        return v > -0.3f ? fmaf(s * v, v, v) : e;
+    }
+}
+// tanh |v| = -m / (m + 2) with m = e^(-2 |v|) - 1
+template <class T> __device__ __forceinline__ float fast_tanh(float v) {
+    const float m = fast_expm1<T>(-2.0f * fabsf(v));
+    return copysignf(-m * __builtin_amdgcn_rcpf(m + 2.0f), v);
+}
+
+template <class T, int N> __device__ __forceinline__ void layer_act(int act, float* v) {
     switch (act) {
         case ACT_SIGMOID:
 #pragma unroll
@@ -71,7 +95,7 @@ template <int N> __device__ __forceinline__ void layer_act(int act, float* v) {
             break;
         case ACT_TANH:
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = tanhf(v[j]);
+            for (int j = 0; j < N; ++j) v[j] = fast_tanh<T>(v[j]);
             break;
         case ACT_RELU:
 #pragma unroll
@@ -79,7 +103,7 @@ template <int N> __device__ __forceinline__ void layer_act(int act, float* v) {
             break;
         case ACT_ELU:
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = v[j] > 0.0f ? v[j] : expm1f(v[j]);
+            for (int j = 0; j < N; ++j) v[j] = v[j] > 0.0f ? v[j] : fast_expm1<T>(v[j]);
             break;
         default: break;
     }
@@ -112,12 +136,33 @@ template <class T> __device__ __forceinline__ int pack_scale(uint32_t top_bits) 
     if ((top_bits & 0x7fffffu) > 0x7e0000u) ++e;                              // over 127 * 2^e
     return (e < PackRange<T>::lo ? PackRange<T>::lo : e) + 127;
 }
-template <class T> __device__ __forceinline__ int pack_value(float x, int byte) {
-    if (byte == 255) return 0;
-    const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);          // 2^-e, a normal number for e in [-126, 122]
-    const float q = __builtin_rintf(x * inv);
-    const float lim = byte == PackRange<T>::hi + 127 ? 63.0f : 127.0f;        // 64 * 2^hi would be an infinity of T
-    return (int)fminf(fmaxf(q, -lim), lim);
+// bits of the largest magnitude of N values
+template <int N> __device__ __forceinline__ uint32_t pack_top(const float* f) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) { const uint32_t b = __float_as_uint(f[j]) & 0x7fffffffu; top = top > b ? top : b; }
+    return top;
+}
+// the eight q of a block with that scale byte.  x * 2^-e is exact, and adding 1.5 * 2^23 rounds it to a whole number, halves to
+// even, whose two's complement is the low byte of the sum's bits.  |q| <= 127 by the choice of e.
+template <class T> __device__ __forceinline__ u32x2 pack_bytes(const float (&f)[8], int byte) {
+    const float magic = 12582912.0f;
+    // 2^-e, a normal number for e in [-126, 122]; a block that stands for NaN has q = 0
+    const float inv = byte == 255 ? 0.0f : __uint_as_float((uint32_t)(254 - byte) << 23);
+    uint32_t b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(fmaf(f[j], inv, magic));
+    if (byte == PackRange<T>::hi + 127) {                                     // 64 * 2^hi would be an infinity of T
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(fminf(fmaxf(__uint_as_float(b[j]), magic - 63.0f), magic + 63.0f));
+    }
+    u32x2 w;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t lo = __builtin_amdgcn_perm(b[4 * h + 1], b[4 * h], 0x0c0c0400u), up = __builtin_amdgcn_perm(b[4 * h + 3], b[4 * h + 2], 0x04000c0cu);
+        w[h] = byte == 255 ? 0u : lo | up;
+    }
+    return w;
 }
 __device__ __forceinline__ float unpack_scale(int byte) {
     return byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)byte << 23);
@@ -129,19 +174,14 @@ __device__ __forceinline__ void unpack8(u32x2 q, float scale, float (&f)[8]) {
 // Four neighbouring lanes hold a block (8 columns each; columns behind the row's end are zero): writes its 8 bytes of q and,
 // from the first of the four, the scale byte.
 template <class T> __device__ __forceinline__ void pack_block(const float (&f)[8], int lane, bool store, int8_t* q, uint8_t* scale) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) { const uint32_t b = __float_as_uint(f[j]) & 0x7fffffffu; top = top > b ? top : b; }
+    uint32_t top = pack_top<8>(f);
 #pragma unroll
     for (int d = 1; d <= 2; d <<= 1) { const uint32_t o = (uint32_t)__shfl_xor((int)top, d); top = top > o ? top : o; }
     const int byte = pack_scale<T>(top);
-    u32x2 w = {0u, 0u};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w[j / 4] |= ((uint32_t)pack_value<T>(f[j], byte) & 255u) << (8 * (j % 4));
-    if (store) {
-        __builtin_memcpy(q, &w, 8);
-        if ((lane & 3) == 0) *scale = (uint8_t)byte;
-    }
+    const u32x2 w = pack_bytes<T>(f, byte);
+    if (!store) return;
+    __builtin_memcpy(q, &w, 8);
+    if ((lane & 3) == 0) *scale = (uint8_t)byte;
 }
 
 // ---- groups of rows.  ends[g] is where group g's rows end (it begins where g - 1 ends, group 0 at row 0).  The array is

@@ -241,8 +241,7 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gem
     typedef Stage<T, false, B_ALONG ? BN : BK, B_ALONG ? BK : BN, THREADS, B_ALONG> StageB;
     constexpr int PA = StageA::PLANES, PB = StageB::PLANES;
     constexpr int LDS_A = PA * BM * BK, LDS_B = PB * BN * BK, LDS_STEP = LDS_A + LDS_B;
-    constexpr int EPI_LD = WN + 4, EPI_ROWS = WAVES_K > 1 ? WM : 32;
-    constexpr int EPI = WAVES * EPI_ROWS * EPI_LD * 4, MAIN = LDS_STEP * 2 * BUFS;
+    constexpr int EPI_LD = WN + 4, EPI_ROWS = WAVES_K > 1 ? WM : 32, EPI = WAVES * EPI_ROWS * EPI_LD * 4, MAIN = LDS_STEP * 2 * BUFS;
     __shared__ __attribute__((aligned(16))) char smem[EPI > MAIN ? EPI : MAIN];
     half* const lds = (half*)smem;
 
@@ -349,9 +348,9 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gem
                     for (int s = 2; s >= 1; --s)                              // smallest terms first
 #pragma unroll
                         for (int p = 0; p <= s; ++p)
-                            if (p < PA && s - p < PB) low[i][j] = Mfma<half>::mul(a[p][i], b[s - p][j], low[i][j]);
+                            if (p < PA && s - p < PB) low[i][j] = Mfma<half>::mul(b[s - p][j], a[p][i], low[i][j]);
                 }
-                acc[i][j] = Mfma<half>::mul(a[0][i], b[0][j], acc[i][j]);
+                acc[i][j] = Mfma<half>::mul(b[0][j], a[0][i], acc[i][j]);
             }
     };
     if constexpr (BUFS == 1) {
@@ -390,14 +389,20 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gem
     constexpr int PASS_ROWS = WAVES_K > 1 ? WM / WAVES_K : 32, PASSES = WAVES_K > 1 ? 1 : MI;
     constexpr int ROWP = WN / 8, STEPS = PASS_ROWS * ROWP / 64, ROWS_PER = 64 / ROWP;
     static_assert(64 % ROWP == 0 && STEPS > 0 && (WAVES_K == 1 || WAVES_M * WAVES_N == 1), "a lane keeps its columns");
+    // (the products were taken as B^T A^T: a lane has one row and, in four registers next to each other, four columns)
     auto put_sums = [&](int i, float* to) {
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                float v = acc[i][j][r];
-                if constexpr (SPLIT3) { const float w = v + low[i][j][r]; v = __builtin_isfinite(v) ? w : v; }
-                to[((r >> 2) * 8 + (lane >> 5) * 4 + (r & 3)) * EPI_LD + j * 32 + (lane & 31)] = v;
+            for (int q = 0; q < 4; ++q) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x = acc[i][j][4 * q + e];
+                    if constexpr (SPLIT3) { const float y = x + low[i][j][4 * q + e]; x = __builtin_isfinite(x) ? y : x; }
+                    v[e] = x;
+                }
+                *(f32x4*)(to + (lane & 31) * EPI_LD + j * 32 + q * 8 + (lane >> 5) * 4) = v;
             }
     };
     float* const tile = (float*)smem + wave * EPI_ROWS * EPI_LD;
@@ -455,7 +460,7 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gem
             for (int it = 0; it < STEPS; ++it)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[it][j] += bias[j];
-            layer_act<STEPS * 8>(g.act, &v[0][0]);
+            layer_act<T, STEPS * 8>(g.act, &v[0][0]);
             if (rest) {
 #pragma unroll
                 for (int it = 0; it < STEPS; ++it)
@@ -477,7 +482,7 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gem
                     float a[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) a[j] = j < valid ? (float)(T)v[it][j] : 0.0f;      // the 8-bit form of the value in T
-                    pack_block<T>(a, lane, row < m_end && col < ((g.N + PACK_BLOCK - 1) & -PACK_BLOCK), g.q_out + (int64_t)row * g.ldq + col,
+                    pack_block<T>(a, lane, row < m_end && (col & -PACK_BLOCK) < g.N, g.q_out + (int64_t)row * g.ldq + col,
                                   g.q_scale + (int64_t)row * g.ldq_scale + col / PACK_BLOCK);
                 }
                 if (valid > 0) {

@@ -104,7 +104,7 @@ template <class T, int SL> __device__ __forceinline__ void join(const JoinPart& 
     float sum[8] = {};
     if (valid > 0) {
         const float* src = p.slab + slabs.first * p.slab_stride + (int64_t)row * p.cols + col;
-#pragma unroll 4
+#pragma unroll 8
         for (int s = sl; s < slabs.count; s += SL) {
             float v[8];
             load8f(src + s * p.slab_stride, valid, v);
@@ -415,11 +415,13 @@ template <class F> hipError_t by_width(int64_t n, F f) {
     return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
 }
 int norm_rows_per_block(int64_t n) { return n <= 64 ? 32 : n <= 128 ? 16 : n <= 256 ? 8 : n <= 1024 ? 4 : 1; }
-// 1024 workgroups keep enough rows in flight (512: 121 us at 65536 x 1024 bf16); up to four turns of one workgroup are over sooner
-// than the launch that would join two workgroups' sums
+// Workgroups of the forward pass: four turns each, so that weight and bias are read once for them, where that leaves eight a CU
+int norm_forward_blocks(int64_t rows, int per) { return std::max(norm_blocks(rows, per, 2048), norm_blocks(rows, 4 * per, 4096)); }
+// Workgroups of the backward pass: four turns each up to 1024 of them, which keep enough rows in flight (65536 x 1024 bf16: 87 us, with
+// 512 of them 121); one, which needs no join, as long as four turns do.
 int norm_backward_blocks(int64_t rows, int64_t n) {
     const int per = norm_rows_per_block(n);
-    return rows <= 4 * per ? 1 : norm_blocks(rows, per, 1024);
+    return rows <= 4 * per ? 1 : norm_blocks(rows, 4 * per, 1024);
 }
 
 int check_norm(const smrt_layer_norm* p, const char* who) {
@@ -563,7 +565,7 @@ extern "C" int smrt_layer_norm_forward(const smrt_layer_norm* p, void* hip_strea
     return launched(who, by_type(p->dtype, [&](auto t) {
         return by_width(p->n, [&](auto tpr, auto ch) {
             constexpr int TPR = decltype(tpr)::value, THREADS = TPR > 256 ? TPR : 256;
-            hipLaunchKernelGGL((norm_forward_kernel<decltype(t), TPR, decltype(ch)::value>), dim3(norm_blocks(p->rows, THREADS / TPR, 4096)), dim3(THREADS), 0,
+            hipLaunchKernelGGL((norm_forward_kernel<decltype(t), TPR, decltype(ch)::value>), dim3(norm_forward_blocks(p->rows, THREADS / TPR)), dim3(THREADS), 0,
                                (hipStream_t)hip_stream, a);
             return hipGetLastError();
         });
