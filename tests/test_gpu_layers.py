@@ -624,3 +624,64 @@ def test_grouped_larger_tiles(dtype):
         check_dense_backward(g[s], x[s], w[j], a, "sigmoid", dx[s], dw[j], db[j], dtype)
         lo = hi
     assert not y[lo:].any() and not dx[lo:].any()
+
+
+# ------------------------------------------------------------------------------------------------ the classes' decoders
+@pytest.fixture(scope="module")
+def fitted():
+    from smrt_amd.autoencode import VariationalAutoEncoder
+    rs = np.random.RandomState(0)
+    return [VariationalAutoEncoder([40, 24], 5, activation_function="elu", n_epochs=2, batch_size=32, learning_rate=0.01, random_state=i).fit(
+        rs.uniform(size=(70 + 30 * i, 50))) for i in range(3)]
+
+
+def test_class_decoders_match_the_estimators(fitted):
+    """fp32: the same products and activations in another order of summation; 1e-4 is the agreement that all paths of the decoder are held to."""
+    from smrt_amd.autoencode import ClassDecoders
+    d = ClassDecoders(fitted)
+    rs = np.random.RandomState(1)
+    z, ends = rs.normal(size=(90, 5)).astype(np.float32), [20, 20, 85]
+    got = d.decode(torch.from_numpy(z).cuda(), torch.tensor(ends, device="cuda")).cpu().numpy()
+    assert got.shape == (90, 50)
+    np.testing.assert_allclose(got[:20], fitted[0].feed_forward(z[:20]), rtol=1e-4, atol=1e-6)
+    np.testing.assert_allclose(got[20:85], fitted[2].feed_forward(z[20:85]), rtol=1e-4, atol=1e-6)
+
+
+def test_class_decoders_generate_is_the_estimators_generate(fitted):
+    from smrt_amd.autoencode import ClassDecoders
+    counts = [7, 0, 30]
+    got = ClassDecoders(fitted).generate(counts, np.random.RandomState(5), loc=0.1, scale=0.5).cpu().numpy()
+    rs, want = np.random.RandomState(5), []
+    for e, n in zip(fitted, counts):
+        want.append(e.feed_forward(rs.normal(0.1, 0.5, size=(n, 5))) if n else np.zeros((0, 50), np.float32))
+    np.testing.assert_allclose(got, np.concatenate(want), rtol=1e-4, atol=1e-6)
+    with pytest.raises(ValueError):
+        ClassDecoders(fitted).generate([1, 2], np.random.RandomState(0))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+def test_class_decoders_in_16_bits(fitted, dtype):
+    """Against the chain in 64 bits on the rounded weights, with each layer's rounding carried on by the next layer's weights."""
+    from smrt_amd.autoencode import ClassDecoders
+    d = ClassDecoders(fitted, dtype)
+    z = make(np.random.default_rng(2), dtype, 64, 5)
+    ends = [30, 50, 64]
+    got = d.decode(z.cuda(), torch.tensor(ends, device="cuda"))
+    lo = 0
+    for c, hi in enumerate(ends):
+        a, e = z[lo:hi].double(), torch.zeros(hi - lo, 5, dtype=torch.float64)
+        for w, b, act in d.layers:
+            W = w[c].cpu().double()
+            e = e @ W.abs() + product_tol(a.abs() + e, W, W.shape[0]) + 8 * U
+            a = act64(a @ W + b[c].cpu().double(), act)
+            e = e + 8 * U * (1 + a.abs())
+            e = e + half(dtype) * (a.abs() + e) + tiny(dtype)
+        close(got[lo:hi], a, e, "class %d" % c)
+        lo = hi
+
+
+def test_class_decoders_refuse_other_shapes(fitted):
+    from smrt_amd.autoencode import ClassDecoders, VariationalAutoEncoder
+    other = VariationalAutoEncoder(24, 5, n_epochs=1, batch_size=32, random_state=0).fit(np.random.RandomState(0).uniform(size=(40, 50)))
+    with pytest.raises(ValueError):
+        ClassDecoders([fitted[0], other])

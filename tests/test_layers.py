@@ -154,3 +154,14 @@ def test_pack_entries_refuse():
         assert lib.smrt_pack_rows(*bad, None) == -1, (i, v)
         dt, x, ldx, rows, n, q, ldq, s, lds = bad
         assert lib.smrt_unpack_rows(dt, q, ldq, s, lds, rows, n, x, ldx, None) == -1, (i, v)
+
+
+def test_class_decoders_refuse():
+    from sklearn.exceptions import NotFittedError
+    from smrt_amd.autoencode import ClassDecoders, VariationalAutoEncoder
+    with pytest.raises(ValueError):
+        ClassDecoders([])
+    with pytest.raises(ValueError):
+        ClassDecoders([VariationalAutoEncoder(4, 2)], dtype=torch.float64)
+    with pytest.raises(NotFittedError):
+        ClassDecoders([VariationalAutoEncoder(4, 2)])
