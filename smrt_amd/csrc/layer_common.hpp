@@ -19,33 +19,66 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 constexpr int PACK_BLOCK = 32;            // columns of a row that share one scale byte of the 8-bit form
 
 // Rows move in pieces of 8 columns.  The tensors are a user's: rows may start at any element, so the pieces are read and
-// written as memory of the element's own alignment (global loads and stores take any address on gfx950; 16 bytes stay one
-// instruction).  A piece that the row's end cuts goes element by element.
+// written as memory of the element's own alignment (global loads and stores take any address on gfx950 at the same rate; 16
+// bytes stay one instruction).  The piece that a row's end cuts is made of four, two and one elements, whichever there are: a lane of
+// every wave has one, and eight single elements took longer than the rest of the row (450 columns against 448).
 typedef uint32_t Words4 __attribute__((ext_vector_type(4), aligned(2), may_alias));
+typedef uint32_t Words2 __attribute__((ext_vector_type(2), aligned(2), may_alias));
+typedef uint32_t Words1 __attribute__((aligned(2), may_alias));
+typedef uint16_t Halves1 __attribute__((may_alias));
 
 template <class T> __device__ __forceinline__ void load8(const T* __restrict__ p, int valid, T (&v)[8]) {
+    const char* const at = (const char*)p;
+    u32x4 lo = {0u, 0u, 0u, 0u}, up = {0u, 0u, 0u, 0u};
     if (valid >= 8) {
-#pragma unroll
-        for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
-            const u32x4 w = ((const Words4*)p)[h];
-            __builtin_memcpy((char*)v + 16 * h, &w, 16);
+        lo = *(const Words4*)at;
+        if constexpr (sizeof(T) == 4) up = *(const Words4*)(at + 16);
+    } else if (valid > 0) {
+        const bool four = valid & 4, two = valid & 2, one = valid & 1;
+        if constexpr (sizeof(T) == 4) {
+            u32x4 a = {0u, 0u, 0u, 0u};
+            u32x2 b = {0u, 0u};
+            uint32_t c = 0u;
+            if (four) a = *(const Words4*)at;
+            if (two) b = *(const Words2*)(at + (four ? 16 : 0));
+            if (one) c = *(const Words1*)(at + (four ? 16 : 0) + (two ? 8 : 0));
+            const u32x4 rest = {two ? b[0] : c, two ? b[1] : 0u, two ? c : 0u, 0u};
+            lo = four ? a : rest;
+            up = four ? rest : u32x4{0u, 0u, 0u, 0u};
+        } else {
+            u32x2 a = {0u, 0u};
+            uint32_t b = 0u, c = 0u;
+            if (four) a = *(const Words2*)at;
+            if (two) b = *(const Words1*)(at + (four ? 8 : 0));
+            if (one) c = *(const Halves1*)(at + (four ? 8 : 0) + (two ? 4 : 0));
+            const uint32_t r0 = two ? b : c, r1 = two ? c : 0u;
+            lo = u32x4{four ? a[0] : r0, four ? a[1] : r1, four ? r0 : 0u, four ? r1 : 0u};
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < valid ? p[j] : (T)0.0f;
     }
+    __builtin_memcpy(v, &lo, 16);
+    if constexpr (sizeof(T) == 4) __builtin_memcpy((char*)v + 16, &up, 16);
 }
 template <class T> __device__ __forceinline__ void store8(T* p, int valid, const T (&v)[8]) {
+    char* const at = (char*)p;
+    u32x4 lo, up = {0u, 0u, 0u, 0u};
+    __builtin_memcpy(&lo, v, 16);
+    if constexpr (sizeof(T) == 4) __builtin_memcpy(&up, (const char*)v + 16, 16);
     if (valid >= 8) {
-#pragma unroll
-        for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
-            u32x4 w;
-            __builtin_memcpy(&w, (const char*)v + 16 * h, 16);
-            ((Words4*)p)[h] = w;
+        *(Words4*)at = lo;
+        if constexpr (sizeof(T) == 4) *(Words4*)(at + 16) = up;
+    } else if (valid > 0) {
+        const bool four = valid & 4, two = valid & 2, one = valid & 1;
+        if constexpr (sizeof(T) == 4) {
+            const u32x4 rest = four ? up : lo;
+            if (four) *(Words4*)at = lo;
+            if (two) *(Words2*)(at + (four ? 16 : 0)) = u32x2{rest[0], rest[1]};
+            if (one) *(Words1*)(at + (four ? 16 : 0) + (two ? 8 : 0)) = two ? rest[2] : rest[0];
+        } else {
+            const uint32_t r0 = four ? lo[2] : lo[0], r1 = four ? lo[3] : lo[1];
+            if (four) *(Words2*)at = u32x2{lo[0], lo[1]};
+            if (two) *(Words1*)(at + (four ? 8 : 0)) = r0;
+            if (one) *(Halves1*)(at + (four ? 8 : 0) + (two ? 4 : 0)) = (uint16_t)(two ? r1 : r0);
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) if (j < valid) p[j] = v[j];
     }
 }
 template <class T> __device__ __forceinline__ void load8f(const T* __restrict__ p, int valid, float (&f)[8]) {

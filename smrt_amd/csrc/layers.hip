@@ -33,7 +33,14 @@ template <class T, bool PACKED> __global__ void __launch_bounds__(256) dz_kernel
     const Chunk chunk = chunk_rows(p.ends, p.groups, p.rows, blockIdx.x / p.col_blocks, DZ_CHUNK);
     if (chunk.group < 0) return;
     const int lo = chunk.r0, hi = chunk.r1;
-    const int col = cb * 256 + (threadIdx.x & 31) * 8, valid = p.n - col;
+    int col = cb * 256 + (threadIdx.x & 31) * 8, valid = p.n - col, lead = 0;
+    if (!PACKED && valid > 0 && valid < 8 && p.n >= 8) {
+        // the piece that the row's end cuts is the row's last 8 columns instead: its first `lead` are its neighbour's too, who
+        // stores the same values, and only count in the neighbour's sums
+        lead = 8 - valid;
+        col -= lead;
+        valid = 8;
+    }
     float sum[8] = {};
     if (valid > 0) {
         constexpr int U = 4;                       // rows in flight a thread: a row's pieces are a round trip to memory
@@ -70,7 +77,7 @@ template <class T, bool PACKED> __global__ void __launch_bounds__(256) dz_kernel
     }
     if (!p.db) return;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sums[threadIdx.x >> 5][(threadIdx.x & 31) * 8 + j] = sum[j];
+    for (int j = 0; j < 8; ++j) if (j >= lead) sums[threadIdx.x >> 5][(threadIdx.x & 31) * 8 + j - lead] = sum[j];
     __syncthreads();
     const int c = cb * 256 + threadIdx.x;
     if (c < p.n) {
@@ -89,51 +96,62 @@ struct JoinPart {
     const float* slab; int64_t slab_stride;          // slab s at s * slab_stride: [out_rows][cols]
     const int64_t* ends; int32_t groups, rows, chunk;
     int32_t out_rows, cols; void* out; int64_t ld, group_stride;
-    int32_t out_f32, group_blocks, blocks;           // workgroups a group and altogether; 0: nothing to join
+    int32_t out_f32, share, group_blocks, blocks;    // workgroups a group and altogether; 0: nothing to join
 };
-// SL threads share the slabs of a piece of 8 columns: many for the long sums over workgroups, one for the few chunks of a product
-template <class T, int SL> __device__ __forceinline__ void join(const JoinPart& p, int block, float (*lds)[8]) {
-    constexpr int PIECES = 256 / SL;
-    const int group = block / p.group_blocks;
+// A piece of 8 columns has `share` threads (a power of two) that go over its slabs side by side, about eight each, where
+// the pieces alone do not fill the GPU (a gradient of 90 x 113 over 73 slabs: 35 us with a thread a piece, 9 with eight).
+template <class T> __device__ __forceinline__ void join(const JoinPart& p, int block, float (*lds)[8]) {
+    const int pieces = 256 / p.share, group = block / p.group_blocks;
     const Slabs slabs = group_slabs(p.ends, p.groups, p.rows, group, p.chunk);
     if (slabs.count == 1) return;
     const uint32_t per_row = (uint32_t)(p.cols + 7) / 8;
-    const int sl = threadIdx.x / PIECES;
-    const uint32_t piece = (uint32_t)(block - group * p.group_blocks) * PIECES + threadIdx.x % PIECES, row = piece / per_row;
+    const int part = threadIdx.x / pieces, own = threadIdx.x % pieces;
+    const uint32_t piece = (uint32_t)(block - group * p.group_blocks) * pieces + own, row = piece / per_row;
     const int col = (int)(piece - row * per_row) * 8, valid = row < (uint32_t)p.out_rows ? p.cols - col : 0;
+    const float* src = p.slab + slabs.first * p.slab_stride + (int64_t)row * p.cols + col;
     float sum[8] = {};
-    if (valid > 0) {
-        const float* src = p.slab + slabs.first * p.slab_stride + (int64_t)row * p.cols + col;
+    if (valid >= 8) {
 #pragma unroll 8
-        for (int s = sl; s < slabs.count; s += SL) {
+        for (int s = part; s < slabs.count; s += p.share) {
             float v[8];
-            load8f(src + s * p.slab_stride, valid, v);
+            load8(src + s * p.slab_stride, 8, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[j] += v[j];
+        }
+    } else if (valid > 0) {
+        for (int s = part; s < slabs.count; s += p.share) {
+            float v[8];
+            load8(src + s * p.slab_stride, valid, v);
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum[j] += v[j];
         }
     }
-    if constexpr (SL > 1) {
+    if (p.share > 1) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) lds[threadIdx.x][j] = sum[j];
         __syncthreads();
-        if (sl) return;
-        for (int i = 1; i < SL; ++i)
+        if (part) return;
+#pragma unroll 4
+        for (int i = 1; i < p.share; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum[j] += lds[i * PIECES + threadIdx.x][j];
+            for (int j = 0; j < 8; ++j) sum[j] += lds[i * pieces + own][j];
     }
     if (valid <= 0) return;
     const int64_t at = (int64_t)group * p.group_stride + (int64_t)row * p.ld + col;
     if (p.out_f32) store8((float*)p.out + at, valid, sum);
     else store8f((T*)p.out + at, valid, sum);
 }
-template <class T, int SL0, int SL1> __global__ void __launch_bounds__(256) join_kernel(JoinPart a, JoinPart b) {
+template <class T> __global__ void __launch_bounds__(256) join_kernel(JoinPart a, JoinPart b) {
     __shared__ float lds[256][8];
-    if ((int)blockIdx.x < a.blocks) join<T, SL0>(a, blockIdx.x, lds);
-    else join<T, SL1>(b, blockIdx.x - a.blocks, lds);
+    if ((int)blockIdx.x < a.blocks) join<T>(a, blockIdx.x, lds);
+    else join<T>(b, blockIdx.x - a.blocks, lds);
 }
-// fills in group_blocks and blocks; false where that is more than a launch takes
-bool join_blocks(JoinPart& p, int sl) {
-    const int64_t pieces = (int64_t)p.out_rows * ((p.cols + 7) / 8), per = 256 / sl, blocks = (pieces + per - 1) / per;
+// fills in share, group_blocks and blocks; false where that is more than a launch takes
+bool join_blocks(JoinPart& p) {
+    const int64_t slabs = p.rows / ((int64_t)p.chunk * p.groups) + 1, pieces = (int64_t)p.out_rows * ((p.cols + 7) / 8);
+    p.share = 1;
+    while (p.share < 64 && p.share * 8 < slabs && p.share * pieces * p.groups < 65536) p.share *= 2;
+    const int64_t per = 256 / p.share, blocks = (pieces + per - 1) / per;
     if (pieces > 0x7fffffff || blocks * p.groups > 0x3fffffff) return false;
     p.group_blocks = (int32_t)blocks;
     p.blocks = (int32_t)blocks * p.groups;
@@ -537,15 +555,15 @@ extern "C" int smrt_dense_backward(const smrt_dense* p, void* workspace, int64_t
     if (dw && !(p->groups == 1 && !p->ends && p->rows > 0 && p->rows <= b.dw.chunk)) {
         jw = {(const float*)(ws + b.slab_off), p->k * p->n, p->ends, p->groups, (int32_t)p->rows, b.dw.chunk, (int32_t)p->k, (int32_t)p->n, p->dw, p->lddw,
               p->dw_stride, false};
-        if (!join_blocks(jw, 1)) return fail(who, "the weight gradient is too large");
+        if (!join_blocks(jw)) return fail(who, "the weight gradient is too large");
     }
     if (p->db && p->n && !(p->groups == 1 && !p->ends && p->rows > 0 && p->rows <= DZ_CHUNK)) {
         jb = {(const float*)(ws + b.part_off), p->n, p->ends, p->groups, (int32_t)p->rows, DZ_CHUNK, 1, (int32_t)p->n, p->db, 0, p->bias_stride, false};
-        if (!join_blocks(jb, 32)) return fail(who, "the bias gradient is too large");
+        if (!join_blocks(jb)) return fail(who, "the bias gradient is too large");
     }
     if (jw.blocks + jb.blocks == 0) return 0;
     return launched(who, by_type(p->dtype, [&](auto t) {
-        hipLaunchKernelGGL((join_kernel<decltype(t), 1, 32>), dim3(jw.blocks + jb.blocks), dim3(256), 0, stream, jw, jb);
+        hipLaunchKernelGGL((join_kernel<decltype(t)>), dim3(jw.blocks + jb.blocks), dim3(256), 0, stream, jw, jb);
         return hipGetLastError();
     }));
 }
@@ -603,10 +621,10 @@ extern "C" int smrt_layer_norm_backward(const smrt_layer_norm* p, void* workspac
         // slabs of 2 n: the weight's half, then the bias's
         JoinPart jw = {}, jb = {};
         const int32_t n = (int32_t)p->n;
-        if (p->dw) { jw = {a.part, 2 * p->n, nullptr, 1, blocks, 1, 1, n, p->dw, 0, 0, a.w_f32}; join_blocks(jw, 32); }
-        if (p->db) { jb = {a.part + n, 2 * p->n, nullptr, 1, blocks, 1, 1, n, p->db, 0, 0, a.w_f32}; join_blocks(jb, 32); }
+        if (p->dw) { jw = {a.part, 2 * p->n, nullptr, 1, blocks, 1, 1, n, p->dw, 0, 0, a.w_f32}; join_blocks(jw); }
+        if (p->db) { jb = {a.part + n, 2 * p->n, nullptr, 1, blocks, 1, 1, n, p->db, 0, 0, a.w_f32}; join_blocks(jb); }
         e = by_type(p->dtype, [&](auto t) {
-            hipLaunchKernelGGL((join_kernel<decltype(t), 32, 32>), dim3(jw.blocks + jb.blocks), dim3(256), 0, stream, jw, jb);
+            hipLaunchKernelGGL((join_kernel<decltype(t)>), dim3(jw.blocks + jb.blocks), dim3(256), 0, stream, jw, jb);
             return hipGetLastError();
         });
     }

@@ -32,7 +32,9 @@ inline GemmPlan plan_gemm(int layout, bool f32, int64_t rows, int64_t m, int64_t
         if (layout == LAYOUT_DW) {
             // the weight gradient sums over the rows: few tiles, so the rows are cut into chunks, a workgroup a tile and chunk, whose
             // sums are joined afterwards (the slabs pass through memory twice); 512 rows at least, so that a chunk outweighs its slab
-            const int64_t tiles = (m + side[t] - 1) / side[t] * tn, want = std::max<int64_t>((t == TILE_LARGE ? 256 : 512) / std::max<int64_t>(tiles, 1), 1);
+            const int64_t tiles = (m + side[t] - 1) / side[t] * tn, all = (t == TILE_LARGE ? 256 : 512) / std::max<int64_t>(tiles, 1);
+            // one round of the CUs, with the half chunk that a group's end adds on average
+            const int64_t want = std::max<int64_t>({all - (groups > 1 ? (groups + 1) / 2 : 0), all / 2, 1});
             const int64_t chunk = std::max<int64_t>(512, (rows + want - 1) / want + 127) / 128 * 128;
             p.chunk = (int)std::min<int64_t>(chunk, 1 << 30);
             const double chunks = groups == 1 ? (double)((rows + chunk - 1) / chunk) : (double)rows / chunk + 0.5 * groups;
