@@ -252,6 +252,26 @@ template <class F> __device__ __forceinline__ int walk_groups(const int64_t* __r
     }
     return end0;
 }
+// rows of group g
+__device__ __forceinline__ RowSpan group_rows(const int64_t* __restrict__ ends, int n_groups, int rows, int group) {
+    RowSpan s = {group, 0, 0};
+    walk_groups(ends, n_groups, rows, [&](int g, int begin, int end) {
+        const unsigned long long hit = __ballot(g == group);
+        if (hit) { const int f = __builtin_ctzll(hit); s.r0 = __shfl(begin, f); s.r1 = __shfl(end, f); }
+        return hit != 0;
+    });
+    return s;
+}
+// the group of a row, -1 for none
+__device__ __forceinline__ int row_group(const int64_t* __restrict__ ends, int n_groups, int rows, int row) {
+    int group = -1;
+    walk_groups(ends, n_groups, rows, [&](int g, int begin, int end) {
+        const unsigned long long hit = __ballot(begin <= row && row < end);
+        if (hit) group = __shfl(g, __builtin_ctzll(hit));
+        return hit != 0;
+    });
+    return group;
+}
 // the t-th tile of `tile` rows, where no tile crosses from one group into the next; behind the last group come the rows
 // that no group has
 __device__ __forceinline__ RowSpan tile_rows(const int64_t* __restrict__ ends, int n_groups, int rows, int t, int tile) {

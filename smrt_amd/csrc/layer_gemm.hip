@@ -33,7 +33,21 @@ template <class T, int LAYOUT, bool PACKED> static hipError_t run_tile(int tile,
     }
 }
 
+hipError_t LAYER_NAME(const RowsBackward& p, hipStream_t stream) {
+    const int64_t blocks = p.dx_blocks + (p.dw || p.db ? (int64_t)p.groups * p.tiles_k * p.tiles_n : 0);
+    if (blocks <= 0) return hipSuccess;
+    if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((rows_backward_kernel<LAYER_T>), dim3((unsigned)blocks), dim3(ROWS_THREADS), 0, stream, p);
+    return hipGetLastError();
+}
+
 hipError_t LAYER_NAME(int layout, const GemmPlan& p, const GemmArgs& g, hipStream_t stream) {
+    if (p.tile == TILE_ROWS) {
+        GemmArgs r = g;
+        r.tiles_n = (g.N + 63) / 64;
+        hipLaunchKernelGGL((rows_forward_kernel<LAYER_T>), dim3((unsigned)(g.rows * r.tiles_n)), dim3(ROWS_THREADS), 0, stream, r);
+        return hipGetLastError();
+    }
     if (layout == LAYOUT_FORWARD) return run_tile<LAYER_T, LAYOUT_FORWARD, false>(p.tile, g, stream);
     if (layout == LAYOUT_DX) return run_tile<LAYER_T, LAYOUT_DX, false>(p.tile, g, stream);
     return g.A_scale ? run_tile<LAYER_T, LAYOUT_DW, true>(p.tile, g, stream) : run_tile<LAYER_T, LAYOUT_DW, false>(p.tile, g, stream);

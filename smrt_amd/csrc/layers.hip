@@ -384,12 +384,14 @@ hipError_t gemm(int dtype, int layout, const GemmPlan& p, const GemmArgs& g, hip
 }
 
 struct BackwardPlan {
-    bool need_dz, need_sum;
+    bool rows, need_dz, need_sum;
     GemmPlan dw;
     int64_t ld_dz, dz_bytes, slab_off, slab_bytes, part_off, part_bytes, total;
 };
 BackwardPlan plan_backward(const smrt_dense* p) {
     BackwardPlan b = {};
+    b.rows = p->rows && p->n && few_rows(p->dtype == SMRT_F32, p->rows, p->k);
+    if (b.rows) return b;
     const int64_t es = elem_size(p->dtype), G = p->groups;
     b.need_dz = p->activation != SMRT_ACT_IDENTITY && (p->dx || p->dw || p->db);
     b.need_sum = p->db != nullptr;
@@ -407,6 +409,10 @@ BackwardPlan plan_backward(const smrt_dense* p) {
 template <class F> hipError_t by_type(int dtype, F f) {
     return dtype == SMRT_F32 ? f((float)0) : dtype == SMRT_BF16 ? f((bf16)0.0f) : f((f16)0.0f);
 }
+
+hipError_t rows_backward(float, const RowsBackward& r, hipStream_t s) { return layer_gemm_f32(r, s); }
+hipError_t rows_backward(bf16, const RowsBackward& r, hipStream_t s) { return layer_gemm_bf16(r, s); }
+hipError_t rows_backward(f16, const RowsBackward& r, hipStream_t s) { return layer_gemm_f16(r, s); }
 
 template <class T> hipError_t launch_dz(const DzArgs& d, hipStream_t s) {
     const int64_t blocks = (int64_t)d.col_blocks * max_chunks(d.ends != nullptr, d.rows, DZ_CHUNK, d.groups);
@@ -516,13 +522,25 @@ extern "C" int smrt_dense_backward(const smrt_dense* p, void* workspace, int64_t
         return fail(who, "a leading dimension is below its columns");
     if (p->dw && p->groups > 1 && p->dw_stride < span(p->k, p->lddw, p->n)) return fail(who, "the groups' weight gradients overlap");
     const BackwardPlan b = plan_backward(p);
-    if (b.need_dz && p->rows && p->n) {
+    if (p->activation != SMRT_ACT_IDENTITY && p->rows && p->n) {
         if (!p->a) return fail(who, "the activation's value is needed");
         if (packed_a ? p->lda < pad(p->n, PACK_BLOCK) || p->ld_a_scale < (p->n + PACK_BLOCK - 1) / PACK_BLOCK : p->lda < p->n)
             return fail(who, "a leading dimension is below its columns");
     }
     if (p->rows && p->n && !p->grad) return fail(who, "null pointer");
     if (b.total > workspace_bytes || (b.total && !workspace)) return fail(who, "the workspace is smaller than smrt_dense_backward_workspace says");
+    if (b.rows) {
+        RowsBackward r = {};
+        r.grad = p->grad; r.ldg = p->ldg; r.a = p->a; r.lda = p->lda; r.a_scale = p->a_scale; r.ld_a_scale = p->ld_a_scale;
+        r.x = p->x; r.ldx = p->ldx; r.x_scale = p->x_scale; r.ld_x_scale = p->ld_x_scale; r.w = p->w; r.ldw = p->ldw; r.w_stride = p->w_stride;
+        r.dx = p->k ? p->dx : nullptr; r.lddx = p->lddx; r.dw = p->k ? p->dw : nullptr; r.lddw = p->lddw; r.dw_stride = p->dw_stride; r.db = p->db; r.db_stride = p->bias_stride;
+        r.ends = p->ends; r.groups = p->groups; r.rows = (int32_t)p->rows; r.k = (int32_t)p->k; r.n = (int32_t)p->n; r.act = p->activation;
+        const int32_t tiles_k = (int32_t)((p->k + 63) / 64);
+        r.dx_blocks = r.dx ? r.rows * tiles_k : 0;
+        r.tiles_k = r.dw || r.dx ? tiles_k : 1;
+        r.tiles_n = (int32_t)((p->n + 63) / 64);
+        return launched(who, by_type(p->dtype, [&](auto t) { return rows_backward(t, r, stream); }));
+    }
     char* const ws = (char*)workspace;
     const void* dz = p->grad;
     int64_t ld_dz = p->ldg;

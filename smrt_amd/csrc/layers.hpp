@@ -2,7 +2,7 @@
 #pragma once
 #include <algorithm>
 #include <cmath>
-#include "layer_gemm.hpp"
+#include "layer_rows.hpp"
 
 namespace smrt {
 namespace layers {
@@ -11,8 +11,13 @@ namespace layers {
 inline int64_t max_slabs(int64_t rows, int64_t chunk, int64_t groups) { return groups == 1 ? (rows > chunk ? (rows + chunk - 1) / chunk : 0) : rows / chunk + std::min(groups, rows / chunk); }
 inline int64_t max_chunks(bool ends, int64_t rows, int64_t chunk, int64_t groups) { return ends ? max_slabs(rows, chunk, groups) + groups : (rows + chunk - 1) / chunk; }
 
-enum Tile : int { TILE_LARGE = 0, TILE_MEDIUM = 1, TILE_SMALL = 2 };
+enum Tile : int { TILE_LARGE = 0, TILE_MEDIUM = 1, TILE_SMALL = 2, TILE_ROWS = 3 };
 struct GemmPlan { int tile, chunk; };      // chunk: dW's rows a workgroup
+
+// The kernels for a few rows (layer_rows.hpp) read W once per row, so they end where their workgroups, one per row and 64 columns, are
+// two a CU for the 16-bit types and four for fp32.  1024 x 1024, row kernel | 64x64 tile, in us: bf16 1 row 6.8 | 10.8, 32 rows 8.6 | 10.8, 64 rows
+// 12.5 | 10.9; fp32 1 row 7.4 | 24.6, 32 rows 11.5 | 24.7, 64 rows 16.1 | 25.0.
+inline bool few_rows(bool f32, int64_t rows, int64_t columns) { return rows <= 64 && rows * ((columns + 63) / 64) <= (f32 ? 1024 : 512); }
 
 // 16-bit types have 256x256 (8 waves, one workgroup a CU), 128x128 (4 waves, two a CU) and 64x64 tiles whose 4 waves split the
 // summed index; fp32, whose three parts fill the registers sooner, the last two.  A launch takes its share of rounds over the 256 CUs, and at
@@ -23,6 +28,7 @@ struct GemmPlan { int tile, chunk; };      // chunk: dW's rows a workgroup
 inline GemmPlan plan_gemm(int layout, bool f32, int64_t rows, int64_t m, int64_t n, int64_t groups) {
     constexpr int side[3] = {256, 128, 64};
     constexpr double chain[2][3] = {{30, 18.5, 10.5}, {1e9, 54, 24}}, round[2][3] = {{40, 11.7, 5.6}, {1e9, 48, 16}};
+    if (layout == LAYOUT_FORWARD && few_rows(f32, rows, n)) return {TILE_ROWS, 0};
     GemmPlan best = {TILE_SMALL, 512};
     double best_us = 1e30;
     for (int t = f32 ? 1 : 0; t < 3; ++t) {
@@ -51,7 +57,10 @@ inline GemmPlan plan_gemm(int layout, bool f32, int64_t rows, int64_t m, int64_t
 }
 
 hipError_t layer_gemm_f32(int layout, const GemmPlan& p, const GemmArgs& g, hipStream_t stream);
+hipError_t layer_gemm_f32(const RowsBackward& p, hipStream_t stream);
 hipError_t layer_gemm_bf16(int layout, const GemmPlan& p, const GemmArgs& g, hipStream_t stream);
+hipError_t layer_gemm_bf16(const RowsBackward& p, hipStream_t stream);
 hipError_t layer_gemm_f16(int layout, const GemmPlan& p, const GemmArgs& g, hipStream_t stream);
+hipError_t layer_gemm_f16(const RowsBackward& p, hipStream_t stream);
 }  // namespace layers
 }  // namespace smrt

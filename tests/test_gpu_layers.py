@@ -685,3 +685,57 @@ def test_class_decoders_refuse_other_shapes(fitted):
     other = VariationalAutoEncoder(24, 5, n_epochs=1, batch_size=32, random_state=0).fit(np.random.RandomState(0).uniform(size=(40, 50)))
     with pytest.raises(ValueError):
         ClassDecoders([fitted[0], other])
+
+
+ROWS = [(1, 64, 64), (1, 1100, 70), (2, 5, 1030), (7, 700, 9), (20, 513, 300), (32, 130, 1000), (33, 40, 64), (64, 65, 520), (3, 8, 8), (5, 1, 1)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("i", range(len(ROWS)), ids=[str(s) for s in ROWS])
+def test_dense_few_rows(i, dtype):
+    """The kernels for a few rows, at their limits and over several steps of each sum, from tensors and from 8-bit forms."""
+    from smrt_amd.autoencode import dense, dense_backward, pack_rows, unpack_rows
+    m, k, n = ROWS[i]
+    rng = np.random.default_rng(500 + i)
+    act = ACTS[(i + DTYPES.index(dtype)) % 5]
+    x, w, b, r, g = make(rng, dtype, m, k), make(rng, dtype, k, n, scale=k ** -0.5), make(rng, dtype, n), make(rng, dtype, m, n), make(rng, dtype, m, n)
+    put = odd_rows if i % 2 else (lambda v: v.cuda())
+    y, saved = dense(put(x), put(w), b.cuda(), residual=put(r), activation=act, save="activation")
+    check_dense(x, w, b, r, act, y, saved, dtype)
+    y8, p = dense(put(x), put(w), b.cuda(), residual=put(r), activation=act, save="packed")
+    assert torch.equal(y, y8)
+    if p is not None:
+        want = pack_rows(saved)
+        assert torch.equal(p.q, want.q) and torch.equal(p.scale, want.scale)
+    got = dense_backward(put(g), put(x), put(w), saved, activation=act)
+    check_dense_backward(g, x, w, None if saved is None else saved.cpu(), act, *got, dtype)
+    assert all(torch.equal(u, v) for u, v in zip(got, dense_backward(put(g), put(x), put(w), saved, activation=act)))
+    px = pack_rows(put(x))
+    got = dense_backward(put(g), px, put(w), p, activation=act)
+    check_dense_backward(g, unpack_rows(px).cpu(), w, None if p is None else unpack_rows(p).cpu(), act, *got, dtype)
+    only = dense_backward(put(g), px, put(w), p, activation=act, need_x=False, need_weight=False)
+    assert only[0] is None and only[1] is None and torch.equal(only[2], got[2])
+    only = dense_backward(put(g), px, put(w), p, activation=act, need_weight=False, need_bias=False)
+    assert torch.equal(only[0], got[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("m,ends", [(24, [3, 6, 6, 20, 24]), (10, [4, 2, 7]), (1, [0, 1]), (30, [0] * 70 + [30]), (60, list(range(1, 61))), (12, [-3, 1 << 50])])
+def test_grouped_few_rows(m, ends, dtype):
+    from smrt_amd.autoencode import dense_grouped, dense_grouped_backward
+    rng = np.random.default_rng(600)
+    k, n, G = 90, 70, len(ends)
+    x, w, b, g = make(rng, dtype, m, k), make(rng, dtype, G, k, n, scale=k ** -0.5), make(rng, dtype, G, n), make(rng, dtype, m, n)
+    e = torch.tensor(ends, dtype=torch.int64, device="cuda")
+    out = torch.full((m, n), 5.0, dtype=dtype, device="cuda")
+    dense_grouped(x.cuda(), e, w.cuda(), b.cuda(), activation="elu", out=out)
+    y, saved = dense_grouped(x.cuda(), e, w.cuda(), b.cuda(), activation="elu", save="activation")
+    dx, dw, db = dense_grouped_backward(g.cuda(), x.cuda(), e, w.cuda(), saved, activation="elu")
+    lo = 0
+    for j, hi in enumerate(sound_ends(ends, m)):
+        s = slice(lo, hi)
+        check_dense(x[s], w[j], b[j], None, "elu", y[s], None, dtype)
+        check_dense_backward(g[s], x[s], w[j], saved[s].cpu(), "elu", dx[s], dw[j], db[j], dtype)
+        lo = hi
+    assert not y[lo:].any() and not dx[lo:].any()
+    assert torch.equal(out[:lo], y[:lo]) and (out[lo:] == 5.0).all()
