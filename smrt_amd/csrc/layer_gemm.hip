@@ -25,11 +25,9 @@ template <class T, int LAYOUT, bool PACKED> static hipError_t run_tile(int tile,
         if (tile == TILE_SMALL) return run<T, LAYOUT, PACKED, 64, 64, 64, 1, 1, 4, 1>(g, stream);
         return run<T, LAYOUT, PACKED, 128, 128, 32, 2, 2, 1, 1>(g, stream);
     } else {
-        // 256x256: steps of 64 where both operands lie along the summed index (dx: 153 us against 157 at 65536 x 1024 x 1024), of 32
-        // where one is turned (forward: 165 against 180)
-        if (tile == TILE_LARGE) return run<T, LAYOUT, PACKED, 256, 256, LAYOUT == LAYOUT_DX ? 64 : 32, 2, 4, 1, 2>(g, stream);
-        if (tile == TILE_MEDIUM) return run<T, LAYOUT, PACKED, 128, 128, 64, 2, 2, 1, 2>(g, stream);
-        return run<T, LAYOUT, PACKED, 64, 64, 128, 1, 1, 4, 2>(g, stream);
+        if (tile == TILE_LARGE) return run<T, LAYOUT, PACKED, 256, 256, 32, 2, 4, 1, 3>(g, stream);
+        if (tile == TILE_MEDIUM) return run<T, LAYOUT, PACKED, 128, 128, 64, 2, 2, 1, 1>(g, stream);
+        return run<T, LAYOUT, PACKED, 64, 64, 128, 1, 1, 4, 1>(g, stream);
     }
 }
 

@@ -67,32 +67,52 @@ template <class T, bool PACKED, int ROWS, int COLS, int THREADS, bool ALONG> str
     static constexpr int ESZ = PACKED ? 1 : sizeof(T);
     typedef typename Planes<T>::half half;
     static_assert(PIECES % THREADS == 0 && THREADS % CH == 0, "a thread keeps its columns");
+    static constexpr int BACK = 8;                   // columns before the tile's first where the loads' base lies: a piece may begin there
     Raw<T, PACKED> raw[PER];
-    uint32_t off[PER], soff[PACKED ? PER : 1];       // bytes from the tile's first element (of the scale bytes)
-    int shift;                                       // across: elements by which the piece that the row's end cuts is read earlier
+    uint32_t off[PER], soff[PACKED ? PER : 1];       // bytes from the base (of the scale bytes: from the tile's first)
+    int shift;                                       // elements by which a piece that an end cuts is read earlier
 
-    // rows and cols: what the tile has of the matrix along its own index (rows for ALONG, columns otherwise).  Everything else
-    // that a thread loads lies inside for every whole step along the summed index, so those loads need no test: rows behind the
+    // rows and cols: what the tile has of the matrix along its own index (rows for ALONG, columns otherwise).  Nothing else needs a
+    // test: every load stays inside the matrix, so the loop that issues them has no branch and keeps them in flight.  Rows behind the
     // end read the last row and columns behind the end the last ones, which only reaches results that are never stored.
-    // back: how many columns before the tile's first the loads' base lies (a piece read earlier may begin there).
-    __device__ __forceinline__ void init(int64_t ld, int64_t ld_scale, int rows, int cols, int back) {
+    __device__ __forceinline__ void init(int64_t ld, int64_t ld_scale, int rows, int cols) {
         const int row = threadIdx.x / CH;
         int col = (threadIdx.x % CH) * 8;
         shift = 0;
         if (!ALONG && col + 8 > cols) {
             const int c = PACKED ? (cols - 1) & -8 : cols - 8;
-            shift = col < cols ? col - c : 0;
+            shift = !PACKED && col < cols ? col - c : 0;
             col = c;
         }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             int r = row + i * STEP;
             if (ALONG) r = r < rows ? r : rows - 1;
-            off[i] = (uint32_t)r * (uint32_t)ld * ESZ + (uint32_t)(col + back) * ESZ;
+            off[i] = (uint32_t)r * (uint32_t)ld * ESZ + (uint32_t)(col + BACK) * ESZ;
             if constexpr (PACKED) soff[i] = (uint32_t)r * (uint32_t)ld_scale + (uint32_t)col / PACK_BLOCK;
         }
     }
-    // a whole step; base (and scale) are the same in all lanes
+    // before the last step is requested, which has only `has` of its summed indices
+    __device__ __forceinline__ void to_last(int64_t ld, int64_t ld_scale, int has) {
+        const int row = threadIdx.x / CH, col = (threadIdx.x % CH) * 8;
+        if constexpr (ALONG) {
+            if (col + 8 > has) {
+                shift = col < has ? col - (has - 8) : 0;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) off[i] -= (uint32_t)(col - (has - 8)) * ESZ;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int over = row + i * STEP - (has - 1);
+                if (over > 0) {
+                    off[i] -= (uint32_t)over * (uint32_t)ld * ESZ;
+                    if constexpr (PACKED) soff[i] -= (uint32_t)over * (uint32_t)ld_scale;
+                }
+            }
+        }
+    }
+    // a step; base (and scale) are the same in all lanes
     __device__ __forceinline__ void load(const char* base, const uint8_t* scale) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -100,14 +120,13 @@ template <class T, bool PACKED, int ROWS, int COLS, int THREADS, bool ALONG> str
                 __builtin_memcpy(&raw[i].q, base + off[i], 8);
                 raw[i].scale = scale[soff[i]];
             } else {
-                const T* src = (const T*)(base + off[i]);
-                __builtin_memcpy(&raw[i], src, 8 * sizeof(T));
+                __builtin_memcpy(&raw[i], base + off[i], 8 * sizeof(T));
             }
         }
     }
-    // the piece that was read `shift` elements early, moved to its place (what comes in behind it is never used)
+    // pieces that were read `shift` elements early, moved to their place; what comes in behind is zero
     __device__ __forceinline__ void unshift() {
-        if constexpr (!ALONG && !PACKED) {
+        if constexpr (!PACKED) {
             constexpr int W = 2 * sizeof(T);         // words of a piece
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
@@ -129,8 +148,15 @@ template <class T, bool PACKED, int ROWS, int COLS, int THREADS, bool ALONG> str
             }
         }
     }
-    // the last step along the summed index, with tests: rows x cols is what there is of the tile, the rest is zero
-    __device__ __forceinline__ void load_tail(const char* base, const uint8_t* scale, int64_t ld, int64_t ld_scale, int rows, int cols) {
+    // the last step: what lies behind its `has` summed indices becomes zero
+    __device__ __forceinline__ void clear_last(int has) {
+        if (ALONG) unshift();
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (ALONG ? (int)(threadIdx.x % CH) * 8 >= has : (int)(threadIdx.x / CH) + i * STEP >= has) raw[i] = {};
+    }
+    // any step of a matrix of fewer than 8 columns, which has no whole piece: rows x cols is what there is of the tile, the rest is zero
+    __device__ __forceinline__ void load_narrow(const char* base, const uint8_t* scale, int64_t ld, int64_t ld_scale, int rows, int cols) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int row = threadIdx.x / CH + i * STEP, col = (threadIdx.x % CH) * 8, valid = row < rows ? cols - col : 0;
@@ -225,9 +251,9 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// BUFS = 2: while one step of BK is multiplied the next goes from registers into the other half of LDS and the one after
-// it is requested from memory; one barrier a step.  BUFS = 1 (fp32, whose three parts fill LDS): two barriers a step, and the
-// other workgroup of the CU multiplies meanwhile.
+// BUFS = 1: two barriers a step, and the other workgroups of the CU multiply meanwhile (three of 128x128 in the 16-bit types, two in
+// fp32, whose parts fill three times the LDS).  BUFS = 3, for the tile that leaves room for one workgroup a CU: while one step of BK is multiplied the one
+// after the next goes from registers into LDS and the one behind that is requested from memory; one barrier a step.
 // WAVES_K > 1: the waves share a small tile and split each step's summed indices between them; their sums are joined in LDS.
 template <class T, int LAYOUT, bool PACKED_A, int BM, int BN, int BK, int WAVES_M, int WAVES_N, int WAVES_K, int BUFS>
 __global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gemm_kernel(GemmArgs g) {
@@ -293,33 +319,31 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gem
     const char* pb = (const char*)g.B + ((LAYOUT == LAYOUT_DW || rest ? 0 : group) * g.strideB + (B_ALONG ? n0 * g.ldb + k0 : k0 * g.ldb + n0)) * esb;
     const int64_t step_a = (A_ALONG ? BK : BK * g.lda) * esa, step_b = (B_ALONG ? BK : BK * g.ldb) * esb, step_sc = PACKED_A ? BK * g.lds_scale : 0;
     const int m_has = m_end - m0, n_has = g.N - n0;
-    const bool edge_a = !A_ALONG && !PACKED_A && m_has < BM && (m_has & 7), edge_b = !B_ALONG && n_has < BN && (n_has & 7);
-    const int back_a = A_ALONG || PACKED_A || m0 == 0 ? 0 : 8, back_b = B_ALONG || n0 == 0 ? 0 : 8;
-    pa -= back_a * esa;
-    pb -= back_b * esb;
-    // a matrix of fewer than 8 columns has no whole piece: every step is then loaded with tests
-    const int whole = (!A_ALONG && !PACKED_A && g.M < 8) || (!B_ALONG && g.N < 8) ? 0 : (k_end - k0) / BK;
-    sa.init(g.lda, g.lds_scale, m_has, m_has, back_a);
-    sb.init(g.ldb, 0, n_has, n_has, back_b);
-    const int steps = (k_end - k0 + BK - 1) / BK;
-    auto fetch = [&](int t) {
-        if (t < whole) {
-            sa.load(pa, psc);
-            sb.load(pb, nullptr);
-        } else {
-            const int k_has = k_end - k0 - t * BK;
-            sa.load_tail(pa + back_a * esa, psc, g.lda, g.lds_scale, A_ALONG ? m_has : k_has, A_ALONG ? k_has : m_has);
-            sb.load_tail(pb + back_b * esb, nullptr, g.ldb, 0, B_ALONG ? n_has : k_has, B_ALONG ? k_has : n_has);
+    const int steps = (k_end - k0 + BK - 1) / BK, last_has = k_end - k0 - (steps - 1) * BK;
+    const bool partial = last_has < BK;              // of the summed index, the last step
+    // a piece that an end cuts reaches back over at most 8 columns; a matrix that has not so many is loaded with tests
+    const bool narrow = ((A_ALONG ? g.K : g.M) < 8 && !PACKED_A) || (B_ALONG ? g.K : g.N) < 8;
+    int fetched = 0;
+    // requests the next step, or the last one again (its pieces then go into a part of LDS that nothing reads)
+    auto fetch = [&] {
+        if (partial && fetched == steps - 1) {
+            sa.to_last(g.lda, g.lds_scale, last_has);
+            sb.to_last(g.ldb, 0, last_has);
         }
-        pa += step_a;
-        pb += step_b;
-        if (PACKED_A) psc += step_sc;
+        sa.load(pa - StageA::BACK * esa, psc);
+        sb.load(pb - StageB::BACK * esb, nullptr);
+        asm volatile("" ::: "memory");               // the loads stay here: what uses them is a step away, and the compiler would move them there
+        const bool more = ++fetched < steps;
+        pa += more ? step_a : 0;
+        pb += more ? step_b : 0;
+        if (PACKED_A) psc += more ? step_sc : 0;
     };
-    auto put = [&](int t, half* to) {
-        if (t < whole) {
-            if (edge_a) sa.unshift();
-            if (edge_b) sb.unshift();
+    auto put = [&](int t, half* to, auto edge) {
+        if constexpr (decltype(edge)::value) {
+            if (!A_ALONG) sa.unshift();
+            if (!B_ALONG) sb.unshift();
         }
+        if (partial && t == steps - 1) { sa.clear_last(last_has); sb.clear_last(last_has); }
         sa.store(to);
         sb.store(to + LDS_A);
     };
@@ -353,32 +377,67 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gem
                 acc[i][j] = Mfma<half>::mul(b[0][j], a[0][i], acc[i][j]);
             }
     };
-    if constexpr (BUFS == 1) {
-        if (steps) fetch(0);
-        for (int t = 0; t < steps; ++t) {
-            lds_barrier();
-            put(t, lds);
-            lds_barrier();
-            if (t + 1 < steps) fetch(t + 1);
+    auto run = [&](auto edge) {
+        sa.init(g.lda, g.lds_scale, m_has, m_has);
+        sb.init(g.ldb, 0, n_has, n_has);
+        fetch();
+        if constexpr (BUFS == 1) {
+            for (int t = 0; t < steps; ++t) {
+                lds_barrier();
+                put(t, lds, edge);
+                lds_barrier();
+                fetch();
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) { read(lds, ks); multiply(ks); }
-        }
-    } else {
-        if (steps) { fetch(0); put(0, lds); }
-        if (steps > 1) fetch(1);
-        for (int t = 0; t < steps; ++t) {
-            const half* cur = lds + (t & 1) * LDS_STEP;
+                for (int ks = 0; ks < KS; ++ks) { read(lds, ks); multiply(ks); }
+            }
+        } else {
+            // Three parts of LDS go round: step t multiplies part t, the first operands of step t + 1 are read from the next part before
+            // step t ends, the third is filled from the registers, which then request the step behind it.  The one barrier of a
+            // step is met with operands in hand.
+            static_assert(KS % 2 == 0, "the operands' two sets of registers alternate");
+            half *cur = lds, *next = lds + LDS_STEP, *third = lds + 2 * LDS_STEP;
+            put(0, cur, edge);
+            fetch();
+            put(1, next, edge);
+            fetch();
             lds_barrier();
             read(cur, 0);
+            for (int t = 0; t < steps; ++t) {
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                if (ks + 1 < KS) read(cur, ks + 1);
-                multiply(ks);
-                if (ks == 0 && t + 1 < steps) {
-                    put(t + 1, lds + ((t + 1) & 1) * LDS_STEP);
-                    if (t + 2 < steps) fetch(t + 2);
+                for (int ks = 0; ks < KS; ++ks) {
+                    if (ks + 1 < KS) read(cur, ks + 1);
+                    else read(next, 0);
+                    multiply(ks);
+                    if (ks == 0) {
+                        put(t + 2, third, edge);
+                        fetch();
+                    }
                 }
+                lds_barrier();
+                half* const free = cur;
+                cur = next;
+                next = third;
+                third = free;
             }
+        }
+    };
+    if (steps > 0) {
+        if (narrow) {
+            for (int t = 0; t < steps; ++t) {
+                const int k_has = k_end - k0 - t * BK;
+                lds_barrier();
+                sa.load_narrow(pa + t * step_a, psc + t * step_sc, g.lda, g.lds_scale, A_ALONG ? m_has : k_has, A_ALONG ? k_has : m_has);
+                sb.load_narrow(pb + t * step_b, nullptr, g.ldb, 0, B_ALONG ? n_has : k_has, B_ALONG ? k_has : n_has);
+                sa.store(lds);
+                sb.store(lds + LDS_A);
+                lds_barrier();
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) { read(lds, ks); multiply(ks); }
+            }
+        } else if ((!A_ALONG && m_has < BM && (m_has & 7)) || (!B_ALONG && n_has < BN && (n_has & 7))) {
+            run(std::true_type());
+        } else {
+            run(std::false_type());
         }
     }
 
