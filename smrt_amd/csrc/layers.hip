@@ -126,16 +126,16 @@ template <class T> __device__ __forceinline__ void join(const JoinPart& p, int b
             for (int j = 0; j < 8; ++j) sum[j] += v[j];
         }
     }
-    if (p.share > 1) {
+    for (int half = p.share / 2; half; half /= 2) {
+        if (part >= half && part < 2 * half)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) lds[threadIdx.x][j] = sum[j];
+            for (int j = 0; j < 8; ++j) lds[threadIdx.x][j] = sum[j];
         __syncthreads();
-        if (part) return;
-#pragma unroll 4
-        for (int i = 1; i < p.share; ++i)
+        if (part < half)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum[j] += lds[i * pieces + own][j];
+            for (int j = 0; j < 8; ++j) sum[j] += lds[(part + half) * pieces + own][j];
     }
+    if (part) return;
     if (valid <= 0) return;
     const int64_t at = (int64_t)group * p.group_stride + (int64_t)row * p.ld + col;
     if (p.out_f32) store8((float*)p.out + at, valid, sum);
@@ -249,27 +249,50 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_backward_kernel(No
 #pragma unroll
     for (int c = 0; c < CH; ++c) { const int col = (c * TPR + lane) * 8; load_weight<T>(p.weight, p.w_f32, col, p.n - col, 1.0f, w[c]); }
     const float inv_n = 1.0f / (float)p.n;
-    for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < p.rows; row0 += (int64_t)gridDim.x * ROWS) {
-        const int64_t row = row0 + threadIdx.x / TPR;
+    // A row is requested while the one before it is worked on; with 16 waves on a row, which have no registers left for that, at its turn.
+    constexpr bool EARLY = TPR < 1024;
+    T g_in[CH][8], x_in[PACKED ? 1 : CH][8];
+    u32x2 q_in[PACKED ? CH : 1];
+    uint8_t scale_in[PACKED ? CH : 1];
+    float mean_in, rstd_in;
+    auto request = [&](int64_t row) {
         const bool live = row < p.rows;
-        const float mean = live ? p.mean[row] : 0.0f, rstd = live ? p.rstd[row] : 0.0f;
-        float h[CH][8], g[CH][8], s1 = 0.0f, s2 = 0.0f;
+        mean_in = live ? p.mean[row] : 0.0f;
+        rstd_in = live ? p.rstd[row] : 0.0f;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int col = (c * TPR + lane) * 8, valid = live ? p.n - col : 0;
-            load8f((const T*)p.grad + row * p.ldg + col, valid, g[c]);
+            load8((const T*)p.grad + row * p.ldg + col, valid, g_in[c]);
             if constexpr (PACKED) {
-                u32x2 q = {0u, 0u};
-                float scale = 0.0f;
+                q_in[c] = u32x2{0u, 0u};
+                scale_in[c] = 0;
                 if (valid > 0) {
-                    __builtin_memcpy(&q, (const int8_t*)p.x + row * p.ldx + col, 8);
-                    scale = unpack_scale(p.x_scale[row * p.ld_x_scale + col / PACK_BLOCK]);
+                    __builtin_memcpy(&q_in[c], (const int8_t*)p.x + row * p.ldx + col, 8);
+                    scale_in[c] = p.x_scale[row * p.ld_x_scale + col / PACK_BLOCK];
                 }
-                unpack8(q, scale, h[c]);
             } else {
-                load8f((const T*)p.x + row * p.ldx + col, valid, h[c]);
+                load8((const T*)p.x + row * p.ldx + col, valid, x_in[c]);
             }
         }
+    };
+    const int64_t first = (int64_t)blockIdx.x * ROWS, stride = (int64_t)gridDim.x * ROWS;
+    if (EARLY) request(first + threadIdx.x / TPR);
+    for (int64_t row0 = first; row0 < p.rows; row0 += stride) {
+        const int64_t row = row0 + threadIdx.x / TPR;
+        const bool live = row < p.rows;
+        if (!EARLY) request(row);
+        const float mean = mean_in, rstd = rstd_in;
+        float h[CH][8], g[CH][8], s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            if constexpr (PACKED) unpack8(q_in[c], unpack_scale(scale_in[c]), h[c]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                g[c][j] = (float)g_in[c][j];
+                if constexpr (!PACKED) h[c][j] = (float)x_in[c][j];
+            }
+        }
+        if (EARLY) request(row + stride);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int valid = live ? p.n - (c * TPR + lane) * 8 : 0;
@@ -441,11 +464,11 @@ template <class F> hipError_t by_width(int64_t n, F f) {
 int norm_rows_per_block(int64_t n) { return n <= 64 ? 32 : n <= 128 ? 16 : n <= 256 ? 8 : n <= 1024 ? 4 : 1; }
 // Workgroups of the forward pass: four turns each, so that weight and bias are read once for them, where that leaves eight a CU
 int norm_forward_blocks(int64_t rows, int per) { return std::max(norm_blocks(rows, per, 2048), norm_blocks(rows, 4 * per, 4096)); }
-// Workgroups of the backward pass: four turns each up to 1024 of them, which keep enough rows in flight (65536 x 1024 bf16: 87 us, with
-// 512 of them 121); one, which needs no join, as long as four turns do.
+// Workgroups of the backward pass: four turns each up to two a CU, which with the next row in flight reach the rate of a copy (65536 x
+// 1024 bf16: 78 us, with four a CU, whose partial sums are twice as many, 87); one, which needs no join, as long as four turns do.
 int norm_backward_blocks(int64_t rows, int64_t n) {
     const int per = norm_rows_per_block(n);
-    return rows <= 4 * per ? 1 : norm_blocks(rows, 4 * per, 1024);
+    return rows <= 4 * per ? 1 : norm_blocks(rows, 4 * per, 512);
 }
 
 int check_norm(const smrt_layer_norm* p, const char* who) {
