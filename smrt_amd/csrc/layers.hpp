@@ -19,15 +19,16 @@ struct GemmPlan { int tile, chunk; };      // chunk: dW's rows a workgroup
 // 12.5 | 10.9; fp32 1 row 7.4 | 24.6, 32 rows 11.5 | 24.7, 64 rows 16.1 | 25.0.
 inline bool few_rows(bool f32, int64_t rows, int64_t columns) { return rows <= 64 && rows * ((columns + 63) / 64) <= (f32 ? 1024 : 512); }
 
-// 16-bit types have 256x256 (8 waves, one workgroup a CU), 128x128 (4 waves, two a CU) and 64x64 tiles whose 4 waves split the
+// 16-bit types have 256x256 (8 waves, one workgroup a CU), 128x128 (4 waves, three a CU) and 64x64 tiles whose 4 waves split the
 // summed index; fp32, whose three parts fill the registers sooner, the last two.  A launch takes its share of rounds over the 256 CUs, and at
 // least as long as one tile's chain of loads and products.  Measured per 1024 summed indices, in us (one tile's chain | a round):
-//             16 bit: 256x256  30 | 40     128x128  18.5 | 11.7     64x64  10.5 | 5.6
-//             fp32:                        128x128  54   | 48       64x64  24   | 16
-// so 65536 x 1024 x 1024 in bf16 took 159 / 186 / 292 us on the three, 4096 x 1024 x 1024 36 / 22 / 25, 1024 x 784 x 450 32 / 21 / 13.
+//             16 bit: 256x256  30 | 40     128x128  17   | 11.7     64x64  10.5 | 5.6
+//             fp32:                        128x128  54   | 45       64x64  24   | 15.5
+// so 65536 x 1024 x 1024 in bf16 took 152 / 155 / 269 us on the three, 4096 x 1024 x 1024 35 / 21 / 25, 40000 x 784 x 450 61 / 51 / 90,
+// 1024 x 784 x 450 28 / 19 / 12; in fp32 65536 x 1024 x 1024 702 / 976 us on the two, 1024 x 784 x 450 48 / 25.
 inline GemmPlan plan_gemm(int layout, bool f32, int64_t rows, int64_t m, int64_t n, int64_t groups) {
     constexpr int side[3] = {256, 128, 64};
-    constexpr double chain[2][3] = {{30, 18.5, 10.5}, {1e9, 54, 24}}, round[2][3] = {{40, 11.7, 5.6}, {1e9, 48, 16}};
+    constexpr double chain[2][3] = {{30, 17, 10.5}, {1e9, 54, 24}}, round[2][3] = {{40, 11.7, 5.6}, {1e9, 45, 15.5}};
     if (layout == LAYOUT_FORWARD && few_rows(f32, rows, n)) return {TILE_ROWS, 0};
     GemmPlan best = {TILE_SMALL, 512};
     double best_us = 1e30;
