@@ -270,9 +270,10 @@ int  smrt_smote_rows_f64(const double* X_dev, int64_t n_x, int64_t ldx, int64_t 
  * the handles above run inside one net, for nets that are put together from layers.
  *
  * Types: SMRT_F32, SMRT_BF16, SMRT_F16; sums are fp32.  Matrices are row-major DEVICE memory, elements of a row next to each
- * other, a leading dimension (in elements, at most 2^21 for what a product reads) for each; rows may start at any element.  Work is queued on hip_stream, nothing is
- * allocated, nothing waits: the calls can be captured into a graph.  Workspaces are the caller's, not shared by calls that may
- * run at the same time.  Sizes may be 0.  Returns 0, or -1 (bad argument, nothing was done) or -2 (launch failed).
+ * other, a leading dimension (in elements, at most 2^21 for what a product reads) for each; rows may start at any element.  An output
+ * shares no memory with an input or another output, but where that is said.  Work is queued on hip_stream, nothing is allocated,
+ * nothing waits: the calls can be captured into a graph.  Workspaces are the caller's, not shared by calls that may run at the
+ * same time.  Sizes may be 0.  Returns 0, or -1 (bad argument, nothing was done) or -2 (launch failed).
  *
  * Groups: with `ends` (device, int64[groups]) group g is the rows [ends[g-1], ends[g]) (from row 0 for g = 0) and has its own
  * weight, w + g * w_stride, and bias, bias + g * bias_stride.  The kernels clamp an end to [the one before, rows], so no
@@ -304,7 +305,7 @@ typedef struct smrt_dense {
     void* dw; int64_t lddw, dw_stride;
     void* db;
 } smrt_dense;
-/* y = act(x W + b) + residual.  y may be the residual itself, and overlaps no other input. */
+/* y = act(x W + b) + residual.  y may be the residual itself. */
 int     smrt_dense_forward(const smrt_dense* args, void* hip_stream);
 /* From grad: dz = grad * act'(.) taken at the value of a (not read for SMRT_ACT_IDENTITY), dx = dz W^T, dw = x^T dz, db = column
  * sums of dz.  The residual's gradient is grad.  A 16-bit dz is rounded once to dtype, as a product's operand. */

@@ -1,6 +1,7 @@
 // The layer operators of the C ABI (include/smrt_hip.h: smrt_dense_*, smrt_layer_norm_*, smrt_pack_rows, smrt_unpack_rows):
 // argument checks, workspaces, launches, and the kernels beside the products (layer_gemm.hpp).
 #include <algorithm>
+#include <initializer_list>
 #include <string>
 #include "layers.hpp"
 #include "../../include/smrt_hip.h"
@@ -379,11 +380,31 @@ int launched(const char* who, hipError_t e) { return e == hipSuccess ? 0 : smrt_
 int elem_size(int dtype) { return dtype == SMRT_F32 ? 4 : 2; }
 int64_t pad(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return a && b && x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
-}
 int64_t span(int64_t rows, int64_t ld, int64_t cols) { return rows > 0 ? (rows - 1) * ld + cols : 0; }
+// What a matrix occupies: `row` bytes every `pitch` bytes (pitch 0: one piece).
+struct Span { const void* p; int64_t bytes, pitch, row; };
+Span matrix(const void* p, int64_t rows, int64_t ld, int64_t cols, int64_t es) { return {p, span(rows, ld, cols) * es, ld * es, cols * es}; }
+Span piece(const void* p, int64_t bytes) { return {p, bytes, 0, bytes}; }
+bool overlap(const Span& a, const Span& b) {
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    if (!x || !y || a.bytes <= 0 || a.row <= 0 || b.bytes <= 0 || b.row <= 0 || x >= y + (uintptr_t)b.bytes || y >= x + (uintptr_t)a.bytes) return false;
+    if (a.pitch <= 0 || a.pitch != b.pitch) return true;
+    // rows of the same pitch may be different columns of one buffer
+    const int64_t from_a = (int64_t)((y > x ? y - x : a.pitch - (x - y) % a.pitch) % a.pitch);
+    return from_a < a.row || from_a + b.row > a.pitch;
+}
+// whether an output shares memory with an input or with another output
+bool any_overlap(std::initializer_list<Span> outs, std::initializer_list<Span> ins) {
+    for (const Span* o = outs.begin(); o != outs.end(); ++o) {
+        for (const Span& i : ins) if (overlap(*o, i)) return true;
+        for (const Span* q = o + 1; q != outs.end(); ++q) if (overlap(*o, *q)) return true;
+    }
+    return false;
+}
+
+Span weights(const void* p, int64_t groups, int64_t stride, int64_t k, int64_t ld, int64_t n, int64_t es) {
+    return groups == 1 ? matrix(p, k, ld, n, es) : piece(p, ((groups - 1) * stride + span(k, ld, n)) * es);
+}
 
 int check_dense(const smrt_dense* p, const char* who) {
     if (!p) return fail(who, "null argument");
@@ -495,6 +516,8 @@ int check_pack(const char* who, int dtype, const void* x, int64_t ldx, int64_t r
     if (rows < 0 || rows > MAX_ROWS || n < 0 || n > MAX_COLS) return fail(who, "bad sizes");
     if (ldx < n || ldq < pad(n, PACK_BLOCK) || ld_scale < (n + PACK_BLOCK - 1) / PACK_BLOCK) return fail(who, "a leading dimension is below its columns");
     if (rows && n && (!x || !q || !scale)) return fail(who, "null pointer");
+    if (any_overlap({matrix(x, rows, ldx, n, elem_size(dtype)), matrix(q, rows, ldq, pad(n, PACK_BLOCK), 1), matrix(scale, rows, ld_scale, (n + PACK_BLOCK - 1) / PACK_BLOCK, 1)}, {}))
+        return fail(who, "the matrix and its 8-bit form overlap");
     return 0;
 }
 constexpr int64_t SMALL_INDEX = 0xffffffffll - 256 * 256 * 64;       // an index and the grid's stride stay below 2^32
@@ -515,11 +538,15 @@ extern "C" int smrt_dense_forward(const smrt_dense* p, void* hip_stream) {
         return fail(who, "a leading dimension is below its columns");
     if (p->rows == 0 || p->n == 0) return 0;
     if (!p->y) return fail(who, "null pointer");
-    const int64_t es = elem_size(p->dtype), y_bytes = span(p->rows, p->ldy, p->n) * es;
-    if (overlap(p->y, y_bytes, p->x, span(p->rows, p->ldx, p->k) * es) ||
-        overlap(p->y, y_bytes, p->w, ((p->groups - 1) * p->w_stride + span(p->k, p->ldw, p->n)) * es) ||
-        (p->residual && (p->residual != p->y || p->ldr != p->ldy) && overlap(p->y, y_bytes, p->residual, span(p->rows, p->ldr, p->n) * es)))
-        return fail(who, "y overlaps an input (it may only be the residual itself)");
+    const int64_t es = elem_size(p->dtype);
+    const int64_t blocks = (p->n + PACK_BLOCK - 1) / PACK_BLOCK;
+    const Span y = matrix(p->y, p->rows, p->ldy, p->n, es), residual = matrix(p->residual, p->rows, p->ldr, p->n, es);
+    const Span a = p->a_scale ? matrix(p->a, p->rows, p->lda, blocks * PACK_BLOCK, 1) : matrix(p->a, p->rows, p->lda, p->n, es);
+    const bool in_place = p->residual == p->y && p->ldr == p->ldy;
+    if (any_overlap({y, a, matrix(p->a ? p->a_scale : nullptr, p->rows, p->ld_a_scale, blocks, 1)},
+                    {matrix(p->x, p->rows, p->ldx, p->k, es), weights(p->w, p->groups, p->w_stride, p->k, p->ldw, p->n, es), in_place ? Span{} : residual}) ||
+        overlap(a, residual))
+        return fail(who, "an output overlaps an input or another output (y may only be the residual itself)");
     GemmArgs g = {};
     g.A = p->x; g.lda = p->ldx; g.B = p->w; g.ldb = p->ldw; g.strideB = p->w_stride; g.C = p->y; g.ldc = p->ldy;
     g.bias = p->bias; g.stride_bias = p->bias_stride; g.residual = p->residual; g.ldr = p->ldr;
@@ -551,6 +578,13 @@ extern "C" int smrt_dense_backward(const smrt_dense* p, void* workspace, int64_t
             return fail(who, "a leading dimension is below its columns");
     }
     if (p->rows && p->n && !p->grad) return fail(who, "null pointer");
+    const int64_t es = elem_size(p->dtype);
+    const bool reads_a = p->activation != SMRT_ACT_IDENTITY;
+    if (any_overlap({matrix(p->dx, p->rows, p->lddx, p->k, es), weights(p->dw, p->groups, p->dw_stride, p->k, p->lddw, p->n, es),
+                     piece(p->db, ((p->groups - 1) * p->bias_stride + p->n) * es), piece(workspace, b.total)},
+                    {matrix(p->grad, p->rows, p->ldg, p->n, es), weights(p->w, p->groups, p->w_stride, p->k, p->ldw, p->n, es),
+                     matrix(p->x, p->rows, p->ldx, p->k, p->x_scale ? 1 : es), matrix(reads_a ? p->a : nullptr, p->rows, p->lda, p->n, packed_a ? 1 : es)}))
+        return fail(who, "an output or the workspace overlaps an input or another output");
     if (b.total > workspace_bytes || (b.total && !workspace)) return fail(who, "the workspace is smaller than smrt_dense_backward_workspace says");
     if (b.rows) {
         RowsBackward r = {};
@@ -618,8 +652,11 @@ extern "C" int smrt_layer_norm_forward(const smrt_layer_norm* p, void* hip_strea
     if (!p->y) return fail(who, "null pointer");
     if (!(p->eps >= 0.0f)) return fail(who, "eps must be >= 0");
     const int64_t es = elem_size(p->dtype);
-    if ((p->x != p->y || p->ldx != p->ldy) && overlap(p->y, span(p->rows, p->ldy, p->n) * es, p->x, span(p->rows, p->ldx, p->n) * es))
+    if ((p->x != p->y || p->ldx != p->ldy) && overlap(matrix(p->y, p->rows, p->ldy, p->n, es), matrix(p->x, p->rows, p->ldx, p->n, es)))
         return fail(who, "y overlaps x (it may only be x itself)");
+    const int64_t ws = p->n * (p->weight_f32 ? 4 : es);
+    if (any_overlap({matrix(p->y, p->rows, p->ldy, p->n, es), piece(p->mean, p->rows * 4), piece(p->rstd, p->rows * 4)}, {piece(p->weight, ws), piece(p->bias, ws)}))
+        return fail(who, "an output overlaps a weight or another output");
     const NormArgs a = norm_args(p);
     return launched(who, by_type(p->dtype, [&](auto t) {
         return by_width(p->n, [&](auto tpr, auto ch) {
@@ -646,6 +683,11 @@ extern "C" int smrt_layer_norm_backward(const smrt_layer_norm* p, void* workspac
         return fail(who, "a leading dimension is below its columns");
     if (p->rows && !p->grad) return fail(who, "null pointer");
     const int64_t need = smrt_layer_norm_backward_workspace(p);
+    const int64_t es = elem_size(p->dtype), ws = p->n * (p->weight_f32 ? 4 : es);
+    if (any_overlap({matrix(p->dx, p->rows, p->lddx, p->n, es), piece(p->dw, ws), piece(p->db, ws), piece(workspace, need)},
+                    {matrix(p->grad, p->rows, p->ldg, p->n, es), matrix(p->x, p->rows, p->ldx, p->n, p->x_scale ? 1 : es), piece(p->weight, ws),
+                     piece(p->mean, p->rows * 4), piece(p->rstd, p->rows * 4)}))
+        return fail(who, "an output or the workspace overlaps an input or another output");
     if (need > workspace_bytes || (need && !workspace)) return fail(who, "the workspace is smaller than smrt_layer_norm_backward_workspace says");
     NormArgs a = norm_args(p);
     const int blocks = norm_backward_blocks(p->rows, p->n);

@@ -739,3 +739,124 @@ def test_grouped_few_rows(m, ends, dtype):
         lo = hi
     assert not y[lo:].any() and not dx[lo:].any()
     assert torch.equal(out[:lo], y[:lo]) and (out[lo:] == 5.0).all()
+
+
+# ------------------------------------------------------------------------------------------------ the ends of what the calls allow
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_columns_of_one_buffer(dtype):
+    """Input and output as different columns of one matrix, with rows that interleave in memory; columns that meet are refused."""
+    from smrt_amd import _hip
+    from smrt_amd.autoencode import dense, layer_norm
+    rng = np.random.default_rng(70)
+    x, w, r = make(rng, dtype, 90, 50), make(rng, dtype, 50, 70, scale=0.2), make(rng, dtype, 90, 70)
+    buf = torch.full((90, 200), 3.0, dtype=dtype, device="cuda")
+    buf[:, :50], buf[:, 120:190] = x.cuda(), r.cuda()
+    dense(buf[:, :50], w.cuda(), residual=buf[:, 120:190], activation="elu", out=buf[:, 50:120])
+    check_dense(x, w, None, r, "elu", buf[:, 50:120], None, dtype)
+    assert torch.equal(buf[:, :50].cpu(), x) and torch.equal(buf[:, 120:190].cpu(), r) and (buf[:, 190:] == 3.0).all()
+    want = layer_norm(x.cuda())[0]
+    layer_norm(buf[:, :50], out=buf[:, 150:])
+    assert torch.equal(buf[:, 150:], want) and torch.equal(buf[:, :50].cpu(), x)
+    for out in (buf[:, 49:119], buf[1:, 49:119]):
+        with pytest.raises(_hip.HipLibraryError):
+            dense(buf[:out.shape[0], :50], w.cuda(), out=out)
+    with pytest.raises(_hip.HipLibraryError):
+        layer_norm(buf[:89, :50], out=buf[1:, :50])
+
+
+WIDTHS = [1, 7, 8, 9, 15, 16, 17, 31, 33, 63, 64, 65, 71, 72, 73, 127, 128, 129, 135]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("k", WIDTHS)
+def test_every_way_a_piece_is_cut(k, dtype):
+    """Widths around the pieces and tiles in both directions, rows between NaN, in forward and backward products."""
+    from smrt_amd.autoencode import dense, dense_backward
+    rng = np.random.default_rng(7000 + k)
+    m = 150
+    x = make(rng, dtype, m, k)
+    for n in WIDTHS:
+        w, g = make(rng, dtype, k, n, scale=k ** -0.5), make(rng, dtype, m, n)
+        y = dense(odd_rows(x), odd_rows(w))
+        check_dense(x, w, None, None, "identity", y, None, dtype)
+        dx, dw, db = dense_backward(odd_rows(g), odd_rows(x), odd_rows(w))
+        check_dense_backward(g, x, w, None, "identity", dx, dw, db, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_widest_strides(dtype):
+    """Rows 2^21 elements apart, the most that the products take: the same bits as from rows next to each other."""
+    from smrt_amd import _hip
+    from smrt_amd.autoencode import dense, dense_backward, layer_norm, pack_rows
+    big = torch.empty((300, 1 << 21), dtype=dtype, device="cuda")
+    gen = torch.Generator().manual_seed(5)
+    put = lambda col, r, c: big[:r, col:col + c].copy_(torch.randn((r, c), generator=gen).to(dtype))
+    x, w, g = put(1, 300, 270), put(400, 270, 261), put((1 << 21) - 261, 300, 261)
+    X, W, G = x.contiguous(), w.contiguous(), g.contiguous()
+    out = big[:, 1000:1261]
+    dense(x, w, activation="tanh", out=out)
+    want = dense(X, W, activation="tanh")
+    assert torch.equal(out, want)
+    for p, q in zip(dense_backward(g, x, w, out, activation="tanh"), dense_backward(G, X, W, want, activation="tanh")):
+        assert torch.equal(p, q)
+    assert torch.equal(layer_norm(x)[0], layer_norm(X)[0])
+    assert torch.equal(pack_rows(x).q, pack_rows(X).q)
+    del big, x, w, g, out
+    wide = torch.zeros((2, (1 << 21) + 8), dtype=dtype, device="cuda")
+    with pytest.raises(_hip.HipLibraryError):
+        dense(wide[:, :8], W[:8])
+
+
+def test_most_groups():
+    """65 535 groups, most of one row, some empty, some of several."""
+    from smrt_amd.autoencode import dense_grouped, dense_grouped_backward
+    G, k, n = 65535, 9, 7
+    gen = torch.Generator().manual_seed(6)
+    sizes = torch.randint(0, 3, (G,), generator=gen)
+    sizes[1000], sizes[G - 1] = 700, 5
+    ends = sizes.cumsum(0)
+    m = int(ends[-1])
+    which = torch.repeat_interleave(torch.arange(G), sizes)
+    x, w, g = torch.randn((m, k), generator=gen), torch.randn((G, k, n), generator=gen), torch.randn((m, n), generator=gen)
+    y = dense_grouped(x.cuda(), ends.cuda(), w.cuda())
+    dx, dw, db = dense_grouped_backward(g.cuda(), x.cuda(), ends.cuda(), w.cuda())
+    X, W, D = x.double(), w.double(), g.double()
+    own = W[which]
+    tol = lambda terms, count: 2 * (count + 10) * U * terms + half(F32) * 2 * terms + tiny(F32)
+    close(y, (X[:, :, None] * own).sum(1), tol((X[:, :, None] * own).abs().sum(1), k), "y")
+    close(dx, (own * D[:, None]).sum(2), tol((own * D[:, None]).abs().sum(2), n), "dx")
+    outer = X[:, :, None] * D[:, None]
+    zero = torch.zeros((G, k, n), dtype=torch.float64)
+    close(dw, zero.index_add(0, which, outer), tol(zero.index_add(0, which, outer.abs()), 700), "dw")
+    zero = torch.zeros((G, n), dtype=torch.float64)
+    close(db, zero.index_add(0, which, D), tol(zero.index_add(0, which, D.abs()), 700), "db")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("m,ends", [(50, [10, 20, 41]), (900, [200, 500, 801])])
+def test_nan_stays_in_its_class(m, ends, dtype):
+    """A class of NaN rows, a class with a NaN weight, and NaN rows of no class leave the others' results as they are."""
+    from smrt_amd.autoencode import dense_grouped, dense_grouped_backward
+    rng = np.random.default_rng(80)
+    k, n = 70, 45
+    x, w, g = make(rng, dtype, m, k), make(rng, dtype, 3, k, n, scale=0.1), make(rng, dtype, m, n)
+    e = torch.tensor(ends, device="cuda")
+
+    def run(x, w, g):
+        y, saved = dense_grouped(x.cuda(), e, w.cuda(), activation="sigmoid", save="activation")
+        return (y, *dense_grouped_backward(g.cuda(), x.cuda(), e, w.cuda(), saved, activation="sigmoid"))
+    want = run(x, w, g)
+    x, w, g = x.clone(), w.clone(), g.clone()
+    x[ends[0]:ends[1]] = float("nan")
+    x[ends[2]:], g[ends[2]:] = float("nan"), float("nan")
+    y, dx, dw, db = run(x, w, g)
+    a, b, c = slice(0, ends[0]), slice(ends[0], ends[1]), slice(ends[1], ends[2])
+    for s in (a, c):
+        assert torch.equal(y[s], want[0][s]) and torch.equal(dx[s], want[1][s])
+    assert y[b].isnan().all() and dx[b].isnan().all() and dw[1].isnan().all() and db[1].isnan().all()
+    for j in (0, 2):
+        assert torch.equal(dw[j], want[2][j]) and torch.equal(db[j], want[3][j])
+    assert not y[ends[2]:].any() and not dx[ends[2]:].any()
+    w[2, 5, 7] = float("nan")
+    y = run(x, w, g)[0]
+    assert torch.equal(y[a], want[0][a]) and y[c, 7].isnan().all() and torch.equal(y[c, :7], want[0][c, :7]) and torch.equal(y[c, 8:], want[0][c, 8:])

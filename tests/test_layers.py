@@ -126,6 +126,8 @@ def test_entries_refuse_null_and_small_workspaces():
     assert lib.smrt_layer_norm_backward(None, None, 0, None) == -1
     assert lib.smrt_layer_norm_backward_workspace(None) == -1
     args = _dense_args()
+    assert lib.smrt_dense_backward_workspace(C.byref(args)) == 0          # a few rows have all their gradients from one launch
+    args = _dense_args(rows=100)
     need = lib.smrt_dense_backward_workspace(C.byref(args))
     assert need > 0
     assert lib.smrt_dense_backward(C.byref(args), 0xa0000, need - 1, None) == -1
@@ -154,6 +156,28 @@ def test_pack_entries_refuse():
         assert lib.smrt_pack_rows(*bad, None) == -1, (i, v)
         dt, x, ldx, rows, n, q, ldq, s, lds = bad
         assert lib.smrt_unpack_rows(dt, q, ldq, s, lds, rows, n, x, ldx, None) == -1, (i, v)
+
+
+def test_entries_refuse_shared_memory():
+    lib = _hip.load()
+    for kw in (dict(a=0x30010), dict(a=0x10000), dict(a=0x20020), dict(residual=0x40000, ldr=16), dict(a_scale=0x30000, lda=32, ld_a_scale=1)):
+        args = _dense_args(**kw)
+        assert lib.smrt_dense_forward(C.byref(args), None) == -1 and b"overlaps" in lib.smrt_last_error(), kw
+    for kw in (dict(dx=0x50000), dict(dx=0x10000), dict(dx=0x40000), dict(dw=0x20000), dict(dw=0x60000), dict(db=0x70000), dict(db=0x50000)):
+        args = _dense_args(**kw)
+        assert lib.smrt_dense_backward(C.byref(args), 0xa0000, 1 << 20, None) == -1 and b"overlaps" in lib.smrt_last_error(), kw
+    args = _dense_args(rows=100)
+    assert lib.smrt_dense_backward(C.byref(args), 0x50000, 1 << 20, None) == -1 and b"overlaps" in lib.smrt_last_error()
+    norm = dict(dtype=1, rows=4000, n=64, eps=1e-5, x=0x10000, ldx=64, weight=0x100000, y=0x200000, ldy=64, mean=0x900000, rstd=0xa00000, grad=0xb00000,
+                ldg=64, dx=0xc00000, lddx=64, dw=0xd00000, db=0xe00000)
+    for kw in (dict(y=0x100000), dict(mean=0x200010), dict(rstd=0x900000)):
+        args = _hip.LayerNorm(**{**norm, **kw})
+        assert lib.smrt_layer_norm_forward(C.byref(args), None) == -1 and b"overlaps" in lib.smrt_last_error(), kw
+    for kw in (dict(dx=0xb00000), dict(dx=0x10000), dict(dw=0x100000), dict(db=0xd00000), dict(db=0x900000)):
+        args = _hip.LayerNorm(**{**norm, **kw})
+        assert lib.smrt_layer_norm_backward(C.byref(args), 0x2000000, 1 << 30, None) == -1 and b"overlaps" in lib.smrt_last_error(), kw
+    assert lib.smrt_pack_rows(0, 0x1000, 40, 4, 40, 0x1000, 64, 0x3000, 2, None) == -1
+    assert lib.smrt_unpack_rows(0, 0x2000, 64, 0x1010, 2, 4, 40, 0x1000, 40, None) == -1
 
 
 def test_class_decoders_refuse():
