@@ -22,10 +22,18 @@ static hipError_t run(const GemmArgs& in, hipStream_t stream) {
 
 template <class T, int LAYOUT, bool PACKED> static hipError_t run_tile(int tile, const GemmArgs& g, hipStream_t stream) {
     if constexpr (sizeof(T) == 4) {
+        // 8 waves a 128x128 tile hide more of each other's waits than 4 where a CU has one tile (8192 x 784 x 450 forward 47 us against 53) and
+        // do as well where it has many (65536 x 1024 x 1024 718 / 713, dx 702 / 700); where both operands are turned they do worse (817 / 723)
         if (tile == TILE_SMALL) return run<T, LAYOUT, PACKED, 64, 64, 64, 1, 1, 4, 1>(g, stream);
-        return run<T, LAYOUT, PACKED, 128, 128, 32, 2, 2, 1, 1>(g, stream);
+        return run<T, LAYOUT, PACKED, 128, 128, 32, 2, LAYOUT == LAYOUT_DW ? 2 : 4, 1, 1>(g, stream);
     } else {
         if (tile == TILE_LARGE) return run<T, LAYOUT, PACKED, 256, 256, 32, 2, 4, 1, 3>(g, stream);
+        if constexpr (LAYOUT != LAYOUT_DW) {
+            // the same with up to a tile a CU (8192 x 784 x 450 forward 17.9 us against 20.0, 1024 x 784 x 450 15.7 / 18.6), but with more of them
+            // 4 waves do better (16384 x 1024 x 1024 45.6 us against 46.8, 65536 x 1024 x 1024 159 / 171)
+            const bool one_a_cu = (int64_t)((g.rows + 127) / 128) * ((g.N + 127) / 128) <= 256;
+            if (tile == TILE_MEDIUM && one_a_cu) return run<T, LAYOUT, PACKED, 128, 128, 64, 2, 4, 1, 1>(g, stream);
+        }
         if (tile == TILE_MEDIUM) return run<T, LAYOUT, PACKED, 128, 128, 64, 2, 2, 1, 1>(g, stream);
         return run<T, LAYOUT, PACKED, 64, 64, 128, 1, 1, 4, 1>(g, stream);
     }

@@ -251,7 +251,7 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// BUFS = 1: two barriers a step, and the other workgroups of the CU multiply meanwhile (three of 128x128 in the 16-bit types, two in
+// BUFS = 1: two barriers a step, and the other workgroups of the CU multiply meanwhile (three of 128x128 with 4 waves in the 16-bit types, two in
 // fp32, whose parts fill three times the LDS).  BUFS = 3, for the tile that leaves room for one workgroup a CU: while one step of BK is multiplied the one
 // after the next goes from registers into LDS and the one behind that is requested from memory; one barrier a step.
 // WAVES_K > 1: the waves share a small tile and split each step's summed indices between them; their sums are joined in LDS.

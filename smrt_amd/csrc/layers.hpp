@@ -19,7 +19,7 @@ struct GemmPlan { int tile, chunk; };      // chunk: dW's rows a workgroup
 // 12.5 | 10.9; fp32 1 row 7.4 | 24.6, 32 rows 11.5 | 24.7, 64 rows 16.1 | 25.0.
 inline bool few_rows(bool f32, int64_t rows, int64_t columns) { return rows <= 64 && rows * ((columns + 63) / 64) <= (f32 ? 1024 : 512); }
 
-// 16-bit types have 256x256 (8 waves, one workgroup a CU), 128x128 (4 waves, three a CU) and 64x64 tiles whose 4 waves split the
+// 16-bit types have 256x256 (8 waves, one workgroup a CU), 128x128 (4 or 8 waves) and 64x64 tiles whose 4 waves split the
 // summed index; fp32, whose three parts fill the registers sooner, the last two.  A launch takes its share of rounds over the 256 CUs, and at
 // least as long as one tile's chain of loads and products.  Measured per 1024 summed indices, in us (one tile's chain | a round):
 //             16 bit: 256x256  30 | 40     128x128  17   | 11.7     64x64  10.5 | 5.6
