@@ -5,14 +5,19 @@
 namespace smrt {
 namespace layers {
 
-template <class T, int LAYOUT, bool PACKED, int BM, int BN, int BK, int WAVES_M, int WAVES_N, int WAVES_K, int BUFS>
-static hipError_t run(const GemmArgs& in, hipStream_t stream) {
-    GemmArgs g = in;
+// fills in tiles_n; as many workgroups as any ends need
+template <int LAYOUT, int BM, int BN> static int64_t workgroups(GemmArgs& g) {
     g.tiles_n = (g.N + BN - 1) / BN;
     const int64_t tiles_m = LAYOUT == LAYOUT_DW ? (int64_t)((g.M + BM - 1) / BM) * max_chunks(g.ends != nullptr, g.rows, g.chunk, g.groups)
                           : g.ends             ? (int64_t)g.rows / BM + g.groups + 1
                                                : (g.rows + BM - 1) / BM;
-    const int64_t blocks = tiles_m * g.tiles_n;
+    return tiles_m * g.tiles_n;
+}
+
+template <class T, int LAYOUT, bool PACKED, int BM, int BN, int BK, int WAVES_M, int WAVES_N, int WAVES_K, int BUFS>
+static hipError_t run(const GemmArgs& in, hipStream_t stream) {
+    GemmArgs g = in;
+    const int64_t blocks = workgroups<LAYOUT, BM, BN>(g);
     if (blocks <= 0) return hipSuccess;
     if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((layer_gemm_kernel<T, LAYOUT, PACKED, BM, BN, BK, WAVES_M, WAVES_N, WAVES_K, BUFS>), dim3((unsigned)blocks),
@@ -45,6 +50,17 @@ hipError_t LAYER_NAME(const RowsBackward& p, hipStream_t stream) {
     if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((rows_backward_kernel<LAYER_T>), dim3((unsigned)blocks), dim3(ROWS_THREADS), 0, stream, p);
     return hipGetLastError();
+}
+
+template <class T, bool PACKED> static hipError_t run_pair(const GemmArgs& in_dx, const GemmArgs& in_dw, hipStream_t stream) {
+    GemmArgs dx = in_dx, dw = in_dw;
+    const int64_t dx_blocks = (workgroups<LAYOUT_DX, 64, 64>(dx) + 7) / 8 * 8, blocks = dx_blocks + workgroups<LAYOUT_DW, 64, 64>(dw);
+    if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((layer_gemm_pair_kernel<T, PACKED, 64, 64, sizeof(T) == 4 ? 64 : 128, 4>), dim3((unsigned)blocks), dim3(256), 0, stream, dx, dw, (int)dx_blocks);
+    return hipGetLastError();
+}
+hipError_t LAYER_NAME(const GemmArgs& dx, const GemmArgs& dw, hipStream_t stream) {
+    return dw.A_scale ? run_pair<LAYER_T, true>(dx, dw, stream) : run_pair<LAYER_T, false>(dx, dw, stream);
 }
 
 hipError_t LAYER_NAME(int layout, const GemmPlan& p, const GemmArgs& g, hipStream_t stream) {

@@ -255,20 +255,23 @@ __device__ __forceinline__ void lds_barrier() {
 // fp32, whose parts fill three times the LDS).  BUFS = 3, for the tile that leaves room for one workgroup a CU: while one step of BK is multiplied the one
 // after the next goes from registers into LDS and the one behind that is requested from memory; one barrier a step.
 // WAVES_K > 1: the waves share a small tile and split each step's summed indices between them; their sums are joined in LDS.
-template <class T, int LAYOUT, bool PACKED_A, int BM, int BN, int BK, int WAVES_M, int WAVES_N, int WAVES_K, int BUFS>
-__global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gemm_kernel(GemmArgs g) {
-    constexpr int WAVES = WAVES_M * WAVES_N * WAVES_K, THREADS = WAVES * 64;
-    constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 32, NI = WN / 32, KS = BK / 16 / WAVES_K;
-    constexpr bool SPLIT3 = Planes<T>::n == 3;
-    constexpr bool A_ALONG = LAYOUT != LAYOUT_DW, B_ALONG = LAYOUT == LAYOUT_DX;
+template <class T, int LAYOUT, bool PACKED_A, int BM, int BN, int BK, int WAVES_M, int WAVES_N, int WAVES_K, int BUFS> struct Product {
+    static constexpr int WAVES = WAVES_M * WAVES_N * WAVES_K, THREADS = WAVES * 64;
+    static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 32, NI = WN / 32, KS = BK / 16 / WAVES_K;
+    static constexpr bool SPLIT3 = Planes<T>::n == 3;
+    static constexpr bool A_ALONG = LAYOUT != LAYOUT_DW, B_ALONG = LAYOUT == LAYOUT_DX;
     typedef typename Planes<T>::half half;
     typedef typename Mfma<half>::frag frag;
     typedef Stage<T, PACKED_A, A_ALONG ? BM : BK, A_ALONG ? BK : BM, THREADS, A_ALONG> StageA;
     typedef Stage<T, false, B_ALONG ? BN : BK, B_ALONG ? BK : BN, THREADS, B_ALONG> StageB;
-    constexpr int PA = StageA::PLANES, PB = StageB::PLANES;
-    constexpr int LDS_A = PA * BM * BK, LDS_B = PB * BN * BK, LDS_STEP = LDS_A + LDS_B;
-    constexpr int EPI_LD = WN + 4, EPI_ROWS = WAVES_K > 1 ? WM : 32, EPI = WAVES * EPI_ROWS * EPI_LD * 4, MAIN = LDS_STEP * 2 * BUFS;
-    __shared__ __attribute__((aligned(16))) char smem[EPI > MAIN ? EPI : MAIN];
+    static constexpr int PA = StageA::PLANES, PB = StageB::PLANES;
+    static constexpr int LDS_A = PA * BM * BK, LDS_B = PB * BN * BK, LDS_STEP = LDS_A + LDS_B;
+    static constexpr int EPI_LD = WN + 4, EPI_ROWS = WAVES_K > 1 ? WM : 32, EPI = WAVES * EPI_ROWS * EPI_LD * 4, MAIN = LDS_STEP * 2 * BUFS;
+    static constexpr int SMEM = EPI > MAIN ? EPI : MAIN;
+    __device__ static __forceinline__ void run(const GemmArgs& g, int block, char* smem);
+};
+template <class T, int LAYOUT, bool PACKED_A, int BM, int BN, int BK, int WAVES_M, int WAVES_N, int WAVES_K, int BUFS>
+__device__ __forceinline__ void Product<T, LAYOUT, PACKED_A, BM, BN, BK, WAVES_M, WAVES_N, WAVES_K, BUFS>::run(const GemmArgs& g, int block, char* smem) {
     half* const lds = (half*)smem;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -279,8 +282,8 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gem
     const int tiles_m = (g.M + BM - 1) / BM;
     const int count = LAYOUT == LAYOUT_DW ? count_chunks(g.ends, g.groups, g.rows, g.chunk) * tiles_m : count_tiles(g.ends, g.groups, g.rows, BM);
     const int total = __builtin_amdgcn_readfirstlane(count) * g.tiles_n;
-    if ((int)blockIdx.x >= total) return;
-    int bid = xcd_tile(blockIdx.x, total);
+    if (block >= total) return;
+    int bid = xcd_tile(block, total);
     const int tn = bid % g.tiles_n;
     bid /= g.tiles_n;
     int m0, m_end, k0 = 0, k_end = g.K, group = 0, slab = -1;
@@ -377,7 +380,7 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gem
                 acc[i][j] = Mfma<half>::mul(b[0][j], a[0][i], acc[i][j]);
             }
     };
-    auto run = [&](auto edge) {
+    auto sum = [&](auto edge) {
         sa.init(g.lda, g.lds_scale, m_has, m_has);
         sb.init(g.ldb, 0, n_has, n_has);
         fetch();
@@ -435,9 +438,9 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gem
                 for (int ks = 0; ks < KS; ++ks) { read(lds, ks); multiply(ks); }
             }
         } else if ((!A_ALONG && m_has < BM && (m_has & 7)) || (!B_ALONG && n_has < BN && (n_has & 7))) {
-            run(std::true_type());
+            sum(std::true_type());
         } else {
-            run(std::false_type());
+            sum(std::false_type());
         }
     }
 
@@ -556,6 +559,23 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gem
         }
         fetch_residual(i + 2);
     }
+}
+
+template <class T, int LAYOUT, bool PACKED_A, int BM, int BN, int BK, int WAVES_M, int WAVES_N, int WAVES_K, int BUFS>
+__global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gemm_kernel(GemmArgs g) {
+    typedef Product<T, LAYOUT, PACKED_A, BM, BN, BK, WAVES_M, WAVES_N, WAVES_K, BUFS> P;
+    __shared__ __attribute__((aligned(16))) char smem[P::SMEM];
+    P::run(g, blockIdx.x, smem);
+}
+// Both gradients of a small layer in one launch: dx in the first workgroups (a multiple of 8, so that the others keep their XCDs), dW in the
+// others.  A launch costs 3.5 us of host time, as much as either product of a mini-batch takes.
+template <class T, bool PACKED_A, int BM, int BN, int BK, int WAVES_K>
+__global__ void __launch_bounds__(WAVES_K * 64, 2) layer_gemm_pair_kernel(GemmArgs dx, GemmArgs dw, int dx_blocks) {
+    typedef Product<T, LAYOUT_DX, false, BM, BN, BK, 1, 1, WAVES_K, 1> X;
+    typedef Product<T, LAYOUT_DW, PACKED_A, BM, BN, BK, 1, 1, WAVES_K, 1> W;
+    __shared__ __attribute__((aligned(16))) char smem[X::SMEM > W::SMEM ? X::SMEM : W::SMEM];
+    if ((int)blockIdx.x < dx_blocks) X::run(dx, blockIdx.x, smem);
+    else W::run(dw, (int)blockIdx.x - dx_blocks, smem);
 }
 
 }  // namespace layers

@@ -18,6 +18,7 @@ constexpr int MAX_GROUPS = 65535;
 // ------------------------------------------------------------------------------------------------ dz = g * act'(a), column sums
 // One pass over g (and a): writes dz for the two products that read it, and sums its columns into db on the way (in fp32, from
 // the values before they are rounded to T).  A workgroup has 256 columns of a chunk of DZ_CHUNK rows (chunk_rows), 8 rows x 4 at a time.
+// (with chunks of 256 rows, which need no join at 256 x 784 x 450, the step's three launches there took 35 us instead of 21)
 constexpr int DZ_CHUNK = 64;
 struct DzArgs {
     const void* grad; int64_t ldg;
@@ -427,6 +428,10 @@ hipError_t gemm(int dtype, int layout, const GemmPlan& p, const GemmArgs& g, hip
     return dtype == SMRT_F32 ? layer_gemm_f32(layout, p, g, s) : dtype == SMRT_BF16 ? layer_gemm_bf16(layout, p, g, s) : layer_gemm_f16(layout, p, g, s);
 }
 
+hipError_t gemm_pair(int dtype, const GemmArgs& dx, const GemmArgs& dw, hipStream_t s) {
+    return dtype == SMRT_F32 ? layer_gemm_f32(dx, dw, s) : dtype == SMRT_BF16 ? layer_gemm_bf16(dx, dw, s) : layer_gemm_f16(dx, dw, s);
+}
+
 struct BackwardPlan {
     bool rows, need_dz, need_sum;
     GemmPlan dw;
@@ -611,20 +616,23 @@ extern "C" int smrt_dense_backward(const smrt_dense* p, void* workspace, int64_t
         d.col_blocks = (int32_t)((p->n + 255) / 256);
         if (hipError_t e = by_type(p->dtype, [&](auto t) { return launch_dz<decltype(t)>(d, stream); }); e != hipSuccess) return launched(who, e);
     }
-    GemmArgs g = {};
-    g.ends = p->ends; g.groups = p->groups; g.keep_rest = p->keep_rest; g.rows = (int32_t)p->rows;
-    if (p->dx && p->rows && p->k) {
-        g.A = dz; g.lda = ld_dz; g.B = p->w; g.ldb = p->ldw; g.strideB = p->w_stride; g.C = p->dx; g.ldc = p->lddx;
-        g.M = (int32_t)p->rows; g.N = (int32_t)p->k; g.K = (int32_t)p->n;
-        if (hipError_t e = gemm(p->dtype, LAYOUT_DX, plan_gemm(LAYOUT_DX, p->dtype == SMRT_F32, p->rows, p->rows, p->k, p->groups), g, stream); e != hipSuccess) return launched(who, e);
+    GemmArgs x = {}, w = {};
+    x.ends = w.ends = p->ends; x.groups = w.groups = p->groups; x.keep_rest = p->keep_rest; x.rows = w.rows = (int32_t)p->rows;
+    x.A = dz; x.lda = ld_dz; x.B = p->w; x.ldb = p->ldw; x.strideB = p->w_stride; x.C = p->dx; x.ldc = p->lddx;
+    x.M = (int32_t)p->rows; x.N = (int32_t)p->k; x.K = (int32_t)p->n;
+    w.A = p->x; w.lda = p->ldx; w.A_scale = p->x_scale; w.lds_scale = p->ld_x_scale; w.B = dz; w.ldb = ld_dz;
+    w.C = p->dw; w.ldc = p->lddw; w.strideC = p->dw_stride; w.slab = (float*)(ws + b.slab_off);
+    w.M = (int32_t)p->k; w.N = (int32_t)p->n; w.K = (int32_t)p->rows; w.chunk = b.dw.chunk;
+    const bool dx = p->dx && p->rows && p->k, dw = p->dw && p->k && p->n;
+    const GemmPlan dx_plan = plan_gemm(LAYOUT_DX, p->dtype == SMRT_F32, p->rows, p->rows, p->k, p->groups);
+    hipError_t e = hipSuccess;
+    if (dx && dw && dx_plan.tile == TILE_SMALL && b.dw.tile == TILE_SMALL) {
+        e = gemm_pair(p->dtype, x, w, stream);
+    } else {
+        if (dx) e = gemm(p->dtype, LAYOUT_DX, dx_plan, x, stream);
+        if (dw && e == hipSuccess) e = gemm(p->dtype, LAYOUT_DW, b.dw, w, stream);
     }
-    const bool dw = p->dw && p->k && p->n;
-    if (dw) {
-        g.A = p->x; g.lda = p->ldx; g.A_scale = p->x_scale; g.lds_scale = p->ld_x_scale; g.B = dz; g.ldb = ld_dz; g.strideB = 0;
-        g.C = p->dw; g.ldc = p->lddw; g.strideC = p->dw_stride; g.slab = (float*)(ws + b.slab_off);
-        g.M = (int32_t)p->k; g.N = (int32_t)p->n; g.K = (int32_t)p->rows; g.chunk = b.dw.chunk;
-        if (hipError_t e = gemm(p->dtype, LAYOUT_DW, b.dw, g, stream); e != hipSuccess) return launched(who, e);
-    }
+    if (e != hipSuccess) return launched(who, e);
     // one group with exactly one chunk has nothing to join; groups may be empty or larger
     JoinPart jw = {}, jb = {};
     if (dw && !(p->groups == 1 && !p->ends && p->rows > 0 && p->rows <= b.dw.chunk)) {
