@@ -246,7 +246,7 @@ def _dense(x, ends, weight, bias, residual, activation, save, out):
         r_ptr = residual.data_ptr()
     if out is None:
         _on_gpu(dev)
-        y, ldy = torch.empty((rows, n), dtype=dtype, device=x.device), n or 1
+        y, ldy = x.new_empty((rows, n)), n or 1
     else:
         y_rows, y_cols, ldy = _matrix(out, "out", dtype, dev)
         if y_rows != rows or y_cols != n:
@@ -261,7 +261,7 @@ def _dense(x, ends, weight, bias, residual, activation, save, out):
         elif residual is None:
             saved = y
         else:
-            saved = torch.empty((rows, n), dtype=dtype, device=x.device)
+            saved = x.new_empty((rows, n))
             a_ptr, lda = saved.data_ptr(), n
     args = _hip.Dense(_DTYPES[dtype], act, rows, k, n, groups, out is not None, None if ends is None else ends.data_ptr(),
                       x.data_ptr(), ldx, None, 0, weight.data_ptr(), ldw, w_stride, b_ptr, bias_stride, r_ptr, ldr, y.data_ptr(), ldy,
@@ -285,9 +285,9 @@ def _dense_backward(grad, x, ends, weight, saved, activation, need_x, need_weigh
             raise ValueError("the gradient of %r needs what the forward pass saved" % activation)
         a_ptr, lda, as_ptr, ld_as = _kept(saved, "saved", rows, n, dtype, dev)
     _on_gpu(dev)
-    dx = torch.empty((rows, k), dtype=dtype, device=device) if need_x else None
-    dw = torch.empty(weight.shape, dtype=dtype, device=device) if need_weight else None
-    db = torch.empty((n,) if ends is None else (groups, n), dtype=dtype, device=device) if need_bias else None
+    dx = grad.new_empty((rows, k)) if need_x else None
+    dw = grad.new_empty(weight.shape) if need_weight else None
+    db = grad.new_empty((n,) if ends is None else (groups, n)) if need_bias else None
     args = _hip.Dense(_DTYPES[dtype], act, rows, k, n, groups, 0, None if ends is None else ends.data_ptr(),
                       x_ptr, ldx, xs_ptr, ld_xs, weight.data_ptr(), ldw, w_stride, None, n, None, 0, None, 0, a_ptr, lda, as_ptr, ld_as,
                       grad.data_ptr(), ldg, dx.data_ptr() if need_x else None, k or 1, dw.data_ptr() if need_weight else None, n or 1, k * n,
@@ -369,7 +369,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
     w_f32, w_ptr, b_ptr = _norm_weight(weight, bias, dtype, dev, n)
     if out is None:
         _on_gpu(dev)
-        y, ldy = torch.empty((rows, n), dtype=dtype, device=device), n
+        y, ldy = x.new_empty((rows, n)), n
     else:
         y_rows, y_cols, ldy = _matrix(out, "out", dtype, dev)
         if y_rows != rows or y_cols != n:
@@ -398,9 +398,9 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, need_x=True, need_weig
     if mean.shape[0] != rows or rstd.shape[0] != rows:
         raise ValueError("mean and rstd must have shape (%d,), got %r and %r" % (rows, tuple(mean.shape), tuple(rstd.shape)))
     _on_gpu(dev)
-    dx = torch.empty((rows, n), dtype=dtype, device=device) if need_x else None
-    dw = torch.empty((n,), dtype=weight.dtype, device=device) if need_weight and weight is not None else None
-    db = torch.empty((n,), dtype=weight.dtype, device=device) if need_bias and weight is not None else None
+    dx = grad.new_empty((rows, n)) if need_x else None
+    dw = weight.new_empty((n,)) if need_weight and weight is not None else None
+    db = weight.new_empty((n,)) if need_bias and weight is not None else None
     args = _hip.LayerNorm(_DTYPES[dtype], w_f32, rows, n, 0.0, x_ptr, ldx, xs_ptr, ld_xs, w_ptr, None, None, 0, mean.data_ptr(), rstd.data_ptr(),
                           grad.data_ptr(), ldg, None if dx is None else dx.data_ptr(), n, None if dw is None else dw.data_ptr(),
                           None if db is None else db.data_ptr())

@@ -52,15 +52,16 @@ hipError_t LAYER_NAME(const RowsBackward& p, hipStream_t stream) {
     return hipGetLastError();
 }
 
-template <class T, bool PACKED> static hipError_t run_pair(const GemmArgs& in_dx, const GemmArgs& in_dw, hipStream_t stream) {
+template <class T, bool PACKED> static hipError_t run_pair(const GemmArgs& in_dx, const GemmArgs& in_dw, const JoinPart& db, hipStream_t stream) {
     GemmArgs dx = in_dx, dw = in_dw;
-    const int64_t dx_blocks = (workgroups<LAYOUT_DX, 64, 64>(dx) + 7) / 8 * 8, blocks = dx_blocks + workgroups<LAYOUT_DW, 64, 64>(dw);
+    const int64_t dx_blocks = (workgroups<LAYOUT_DX, 64, 64>(dx) + 7) / 8 * 8, dw_blocks = workgroups<LAYOUT_DW, 64, 64>(dw), blocks = dx_blocks + dw_blocks + db.blocks;
     if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((layer_gemm_pair_kernel<T, PACKED, 64, 64, sizeof(T) == 4 ? 64 : 128, 4>), dim3((unsigned)blocks), dim3(256), 0, stream, dx, dw, (int)dx_blocks);
+    hipLaunchKernelGGL((layer_gemm_pair_kernel<T, PACKED, 64, 64, sizeof(T) == 4 ? 64 : 128>), dim3((unsigned)blocks), dim3(256), 0, stream, dx, dw, db,
+                       (int)dx_blocks, (int)dw_blocks);
     return hipGetLastError();
 }
-hipError_t LAYER_NAME(const GemmArgs& dx, const GemmArgs& dw, hipStream_t stream) {
-    return dw.A_scale ? run_pair<LAYER_T, true>(dx, dw, stream) : run_pair<LAYER_T, false>(dx, dw, stream);
+hipError_t LAYER_NAME(const GemmArgs& dx, const GemmArgs& dw, const JoinPart& db, hipStream_t stream) {
+    return dw.A_scale ? run_pair<LAYER_T, true>(dx, dw, db, stream) : run_pair<LAYER_T, false>(dx, dw, db, stream);
 }
 
 hipError_t LAYER_NAME(int layout, const GemmPlan& p, const GemmArgs& g, hipStream_t stream) {

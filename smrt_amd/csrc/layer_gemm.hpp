@@ -11,7 +11,7 @@
 // product at 2.6 times its peak rate.  hh is summed apart from the small terms: the small ones keep their bits, and where
 // hh alone is an infinity or NaN (whose parts m, l are NaN) it is the answer.
 #pragma once
-#include "layer_common.hpp"
+#include "layer_join.hpp"
 
 namespace smrt {
 namespace layers {
@@ -567,15 +567,18 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * WAVES_K * 64, 2) layer_gem
     __shared__ __attribute__((aligned(16))) char smem[P::SMEM];
     P::run(g, blockIdx.x, smem);
 }
-// Both gradients of a small layer in one launch: dx in the first workgroups (a multiple of 8, so that the others keep their XCDs), dW in the
-// others.  A launch costs 3.5 us of host time, as much as either product of a mini-batch takes.
-template <class T, bool PACKED_A, int BM, int BN, int BK, int WAVES_K>
-__global__ void __launch_bounds__(WAVES_K * 64, 2) layer_gemm_pair_kernel(GemmArgs dx, GemmArgs dw, int dx_blocks) {
-    typedef Product<T, LAYOUT_DX, false, BM, BN, BK, 1, 1, WAVES_K, 1> X;
-    typedef Product<T, LAYOUT_DW, PACKED_A, BM, BN, BK, 1, 1, WAVES_K, 1> W;
+// Both gradients of a small layer in one launch: dx in the first workgroups (a multiple of 8, so that the others keep their XCDs), then dW,
+// then the join of db's partial sums where dW needs none.  A launch costs 3.5 us of host time, as much as either product of a mini-batch.
+template <class T, bool PACKED_A, int BM, int BN, int BK>
+__global__ void __launch_bounds__(256, 2) layer_gemm_pair_kernel(GemmArgs dx, GemmArgs dw, JoinPart db, int dx_blocks, int dw_blocks) {
+    typedef Product<T, LAYOUT_DX, false, BM, BN, BK, 1, 1, 4, 1> X;
+    typedef Product<T, LAYOUT_DW, PACKED_A, BM, BN, BK, 1, 1, 4, 1> W;
+    static_assert(X::THREADS == 256 && W::THREADS == 256 && X::SMEM >= (int)sizeof(float[256][8]), "join's threads and memory");
     __shared__ __attribute__((aligned(16))) char smem[X::SMEM > W::SMEM ? X::SMEM : W::SMEM];
-    if ((int)blockIdx.x < dx_blocks) X::run(dx, blockIdx.x, smem);
-    else W::run(dw, (int)blockIdx.x - dx_blocks, smem);
+    const int block = blockIdx.x;
+    if (block < dx_blocks) X::run(dx, block, smem);
+    else if (block < dx_blocks + dw_blocks) W::run(dw, block - dx_blocks, smem);
+    else join<T>(db, block - dx_blocks - dw_blocks, (float(*)[8])smem);
 }
 
 }  // namespace layers

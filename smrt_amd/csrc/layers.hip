@@ -91,58 +91,7 @@ template <class T, bool PACKED> __global__ void __launch_bounds__(256) dz_kernel
     }
 }
 
-// ------------------------------------------------------------------------------------------------ joining of partial sums
-// out[group][row][col] = sum over the group's slabs (group_slabs), in their order: the result does not depend on timing.
-// A group of one chunk has its result already, one without rows gets zeros.
-struct JoinPart {
-    const float* slab; int64_t slab_stride;          // slab s at s * slab_stride: [out_rows][cols]
-    const int64_t* ends; int32_t groups, rows, chunk;
-    int32_t out_rows, cols; void* out; int64_t ld, group_stride;
-    int32_t out_f32, share, group_blocks, blocks;    // workgroups a group and altogether; 0: nothing to join
-};
-// A piece of 8 columns has `share` threads (a power of two) that go over its slabs side by side, about eight each, where
-// the pieces alone do not fill the GPU (a gradient of 90 x 113 over 73 slabs: 35 us with a thread a piece, 9 with eight).
-template <class T> __device__ __forceinline__ void join(const JoinPart& p, int block, float (*lds)[8]) {
-    const int pieces = 256 / p.share, group = block / p.group_blocks;
-    const Slabs slabs = group_slabs(p.ends, p.groups, p.rows, group, p.chunk);
-    if (slabs.count == 1) return;
-    const uint32_t per_row = (uint32_t)(p.cols + 7) / 8;
-    const int part = threadIdx.x / pieces, own = threadIdx.x % pieces;
-    const uint32_t piece = (uint32_t)(block - group * p.group_blocks) * pieces + own, row = piece / per_row;
-    const int col = (int)(piece - row * per_row) * 8, valid = row < (uint32_t)p.out_rows ? p.cols - col : 0;
-    const float* src = p.slab + slabs.first * p.slab_stride + (int64_t)row * p.cols + col;
-    float sum[8] = {};
-    if (valid >= 8) {
-#pragma unroll 8
-        for (int s = part; s < slabs.count; s += p.share) {
-            float v[8];
-            load8(src + s * p.slab_stride, 8, v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum[j] += v[j];
-        }
-    } else if (valid > 0) {
-        for (int s = part; s < slabs.count; s += p.share) {
-            float v[8];
-            load8(src + s * p.slab_stride, valid, v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum[j] += v[j];
-        }
-    }
-    for (int half = p.share / 2; half; half /= 2) {
-        if (part >= half && part < 2 * half)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) lds[threadIdx.x][j] = sum[j];
-        __syncthreads();
-        if (part < half)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum[j] += lds[(part + half) * pieces + own][j];
-    }
-    if (part) return;
-    if (valid <= 0) return;
-    const int64_t at = (int64_t)group * p.group_stride + (int64_t)row * p.ld + col;
-    if (p.out_f32) store8((float*)p.out + at, valid, sum);
-    else store8f((T*)p.out + at, valid, sum);
-}
+// ------------------------------------------------------------------------------------------------ joining of partial sums (layer_join.hpp)
 template <class T> __global__ void __launch_bounds__(256) join_kernel(JoinPart a, JoinPart b) {
     __shared__ float lds[256][8];
     if ((int)blockIdx.x < a.blocks) join<T>(a, blockIdx.x, lds);
@@ -428,8 +377,8 @@ hipError_t gemm(int dtype, int layout, const GemmPlan& p, const GemmArgs& g, hip
     return dtype == SMRT_F32 ? layer_gemm_f32(layout, p, g, s) : dtype == SMRT_BF16 ? layer_gemm_bf16(layout, p, g, s) : layer_gemm_f16(layout, p, g, s);
 }
 
-hipError_t gemm_pair(int dtype, const GemmArgs& dx, const GemmArgs& dw, hipStream_t s) {
-    return dtype == SMRT_F32 ? layer_gemm_f32(dx, dw, s) : dtype == SMRT_BF16 ? layer_gemm_bf16(dx, dw, s) : layer_gemm_f16(dx, dw, s);
+hipError_t gemm_pair(int dtype, const GemmArgs& dx, const GemmArgs& dw, const JoinPart& db, hipStream_t s) {
+    return dtype == SMRT_F32 ? layer_gemm_f32(dx, dw, db, s) : dtype == SMRT_BF16 ? layer_gemm_bf16(dx, dw, db, s) : layer_gemm_f16(dx, dw, db, s);
 }
 
 struct BackwardPlan {
@@ -625,14 +574,6 @@ extern "C" int smrt_dense_backward(const smrt_dense* p, void* workspace, int64_t
     w.M = (int32_t)p->k; w.N = (int32_t)p->n; w.K = (int32_t)p->rows; w.chunk = b.dw.chunk;
     const bool dx = p->dx && p->rows && p->k, dw = p->dw && p->k && p->n;
     const GemmPlan dx_plan = plan_gemm(LAYOUT_DX, p->dtype == SMRT_F32, p->rows, p->rows, p->k, p->groups);
-    hipError_t e = hipSuccess;
-    if (dx && dw && dx_plan.tile == TILE_SMALL && b.dw.tile == TILE_SMALL) {
-        e = gemm_pair(p->dtype, x, w, stream);
-    } else {
-        if (dx) e = gemm(p->dtype, LAYOUT_DX, dx_plan, x, stream);
-        if (dw && e == hipSuccess) e = gemm(p->dtype, LAYOUT_DW, b.dw, w, stream);
-    }
-    if (e != hipSuccess) return launched(who, e);
     // one group with exactly one chunk has nothing to join; groups may be empty or larger
     JoinPart jw = {}, jb = {};
     if (dw && !(p->groups == 1 && !p->ends && p->rows > 0 && p->rows <= b.dw.chunk)) {
@@ -644,6 +585,16 @@ extern "C" int smrt_dense_backward(const smrt_dense* p, void* workspace, int64_t
         jb = {(const float*)(ws + b.part_off), p->n, p->ends, p->groups, (int32_t)p->rows, DZ_CHUNK, 1, (int32_t)p->n, p->db, 0, p->bias_stride, false};
         if (!join_blocks(jb)) return fail(who, "the bias gradient is too large");
     }
+    hipError_t e = hipSuccess;
+    if (dx && dw && dx_plan.tile == TILE_SMALL && b.dw.tile == TILE_SMALL) {
+        // where dW has nothing to join, db's join, whose sums are there already, goes along
+        e = gemm_pair(p->dtype, x, w, jw.blocks ? JoinPart{} : jb, stream);
+        if (!jw.blocks) jb.blocks = 0;
+    } else {
+        if (dx) e = gemm(p->dtype, LAYOUT_DX, dx_plan, x, stream);
+        if (dw && e == hipSuccess) e = gemm(p->dtype, LAYOUT_DW, b.dw, w, stream);
+    }
+    if (e != hipSuccess) return launched(who, e);
     if (jw.blocks + jb.blocks == 0) return 0;
     return launched(who, by_type(p->dtype, [&](auto t) {
         hipLaunchKernelGGL((join_kernel<decltype(t)>), dim3(jw.blocks + jb.blocks), dim3(256), 0, stream, jw, jb);

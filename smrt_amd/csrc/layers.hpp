@@ -58,13 +58,13 @@ inline GemmPlan plan_gemm(int layout, bool f32, int64_t rows, int64_t m, int64_t
 }
 
 hipError_t layer_gemm_f32(int layout, const GemmPlan& p, const GemmArgs& g, hipStream_t stream);
-hipError_t layer_gemm_f32(const GemmArgs& dx, const GemmArgs& dw, hipStream_t stream);      // both in 64x64 tiles, one launch
+hipError_t layer_gemm_f32(const GemmArgs& dx, const GemmArgs& dw, const JoinPart& db, hipStream_t stream);      // all in one launch, in 64x64 tiles
 hipError_t layer_gemm_f32(const RowsBackward& p, hipStream_t stream);
 hipError_t layer_gemm_bf16(int layout, const GemmPlan& p, const GemmArgs& g, hipStream_t stream);
-hipError_t layer_gemm_bf16(const GemmArgs& dx, const GemmArgs& dw, hipStream_t stream);      // both in 64x64 tiles, one launch
+hipError_t layer_gemm_bf16(const GemmArgs& dx, const GemmArgs& dw, const JoinPart& db, hipStream_t stream);      // all in one launch, in 64x64 tiles
 hipError_t layer_gemm_bf16(const RowsBackward& p, hipStream_t stream);
 hipError_t layer_gemm_f16(int layout, const GemmPlan& p, const GemmArgs& g, hipStream_t stream);
-hipError_t layer_gemm_f16(const GemmArgs& dx, const GemmArgs& dw, hipStream_t stream);      // both in 64x64 tiles, one launch
+hipError_t layer_gemm_f16(const GemmArgs& dx, const GemmArgs& dw, const JoinPart& db, hipStream_t stream);      // all in one launch, in 64x64 tiles
 hipError_t layer_gemm_f16(const RowsBackward& p, hipStream_t stream);
 }  // namespace layers
 }  // namespace smrt
