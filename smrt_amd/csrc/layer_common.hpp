@@ -253,15 +253,16 @@ template <class F> __device__ __forceinline__ int walk_groups(const int64_t* __r
     }
     return end0;
 }
-// rows of group g
+// rows of group g: it begins at the largest of the ends before its own, a maximum that no lane waits for another in (a workgroup for each of
+// thousands of groups spent most of its time in the scans of walk_groups)
 __device__ __forceinline__ RowSpan group_rows(const int64_t* __restrict__ ends, int n_groups, int rows, int group) {
-    RowSpan s = {group, 0, 0};
-    walk_groups(ends, n_groups, rows, [&](int g, int begin, int end) {
-        const unsigned long long hit = __ballot(g == group);
-        if (hit) { const int f = __builtin_ctzll(hit); s.r0 = __shfl(begin, f); s.r1 = __shfl(end, f); }
-        return hit != 0;
-    });
-    return s;
+    int begin = 0;
+#pragma unroll 4
+    for (int g = (int)(threadIdx.x & 63); g < group; g += 64) { const int e = clamp_end(ends, g, n_groups, rows); begin = e > begin ? e : begin; }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) { const int o = __shfl_xor(begin, d); begin = o > begin ? o : begin; }
+    const int end = clamp_end(ends, group, n_groups, rows);
+    return {group, begin, end > begin ? end : begin};
 }
 // the group of a row, -1 for none
 __device__ __forceinline__ int row_group(const int64_t* __restrict__ ends, int n_groups, int rows, int row) {

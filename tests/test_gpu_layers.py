@@ -860,3 +860,27 @@ def test_nan_stays_in_its_class(m, ends, dtype):
     w[2, 5, 7] = float("nan")
     y = run(x, w, g)[0]
     assert torch.equal(y[a], want[0][a]) and y[c, 7].isnan().all() and torch.equal(y[c, :7], want[0][c, :7]) and torch.equal(y[c, 8:], want[0][c, 8:])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_many_groups_of_few_rows(dtype):
+    """60 rows over 20 000 groups, most of them empty, with ends that fall back and leave the rows."""
+    from smrt_amd.autoencode import dense_grouped, dense_grouped_backward
+    G, m, k, n = 20000, 60, 33, 70
+    rng = np.random.default_rng(90)
+    ends = np.sort(rng.integers(0, m + 1, G))
+    ends[::7] -= 25
+    ends[-3:] = [m - 1, -5, 1 << 40]
+    x, w, g = make(rng, dtype, m, k), torch.randn((G, k, n), generator=torch.Generator().manual_seed(2)).to(dtype), make(rng, dtype, m, n)
+    e = torch.from_numpy(ends).cuda()
+    y = dense_grouped(x.cuda(), e, w.cuda())
+    dx, dw, db = dense_grouped_backward(g.cuda(), x.cuda(), e, w.cuda())
+    used, lo = torch.zeros(G, dtype=torch.bool), 0
+    for j, hi in enumerate(sound_ends(ends.tolist(), m)):
+        if hi > lo:
+            s = slice(lo, hi)
+            used[j] = True
+            check_dense(x[s], w[j], None, None, "identity", y[s], None, dtype)
+            check_dense_backward(g[s], x[s], w[j], None, "identity", dx[s], dw[j], db[j], dtype)
+        lo = hi
+    assert lo == m and not dw[~used.cuda()].any() and not db[~used.cuda()].any()
