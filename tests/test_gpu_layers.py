@@ -884,3 +884,39 @@ def test_many_groups_of_few_rows(dtype):
             check_dense_backward(g[s], x[s], w[j], None, "identity", dx[s], dw[j], db[j], dtype)
         lo = hi
     assert lo == m and not dw[~used.cuda()].any() and not db[~used.cuda()].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16], ids=str)
+def test_two_threads_with_a_stream_each(dtype):
+    """The same calls from two host threads at once, each on its own stream: workspaces and results do not mix."""
+    import threading
+    sets = [block_inputs(dtype, m=m, seed=m) for m in (40, 700)]
+    want = []
+    for x, p, ends, gy in sets:
+        y, kept = block(x, p, ends, True)
+        want.append((y, block_backward(gy, p, ends, kept)))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        x, p, ends, gy = sets[i]
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(30):
+                y, kept = block(x, p, ends, True)
+                got = block_backward(gy, p, ends, kept)
+                if not torch.equal(y, want[i][0]) or not all(torch.equal(got[k], want[i][1][k]) for k in got):
+                    bad.append(i)
+        stream.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
+
+
+def test_class_decoders_without_rows(fitted):
+    from smrt_amd.autoencode import ClassDecoders
+    d = ClassDecoders(fitted)
+    assert d.generate([0, 0, 0], np.random.RandomState(1)).shape == (0, 50)
+    some = d.generate([0, 4, 0], np.random.RandomState(1))
+    assert torch.equal(some, ClassDecoders(fitted[1:2]).generate([4], np.random.RandomState(1)))
