@@ -395,7 +395,7 @@ struct BackwardPlan {
 };
 BackwardPlan plan_backward(const smrt_dense* p) {
     BackwardPlan b = {};
-    b.rows = p->rows && p->n && few_rows(p->dtype == SMRT_F32, p->rows, p->k);
+    b.rows = p->rows && p->n && few_rows_backward(p->dtype == SMRT_F32, p->rows, p->k, p->n, p->groups);
     if (b.rows) return b;
     const int64_t es = elem_size(p->dtype), G = p->groups;
     b.need_dz = p->activation != SMRT_ACT_IDENTITY && (p->dx || p->dw || p->db);
@@ -437,13 +437,14 @@ template <class F> hipError_t by_width(int64_t n, F f) {
     if (n <= 256) return f(std::integral_constant<int, 32>(), std::integral_constant<int, 1>());
     if (n <= 512) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
     if (n <= 1024) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
-    if (n <= 2048) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
+    if (n <= 1536) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 3>());
+    if (n <= 2048) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
     if (n <= 4096) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
     if (n <= 8192) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
     if (n <= 16384) return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
     return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
 }
-int norm_rows_per_block(int64_t n) { return n <= 64 ? 32 : n <= 128 ? 16 : n <= 256 ? 8 : n <= 1024 ? 4 : 1; }
+int norm_rows_per_block(int64_t n) { return n <= 64 ? 32 : n <= 128 ? 16 : n <= 256 ? 8 : n <= 2048 ? 4 : 1; }
 // Workgroups of the forward pass: four turns each, so that weight and bias are read once for them, where that leaves eight a CU
 int norm_forward_blocks(int64_t rows, int per) { return std::max(norm_blocks(rows, per, 2048), norm_blocks(rows, 4 * per, 4096)); }
 // Workgroups of the backward pass: four turns each up to two a CU, which with the next row in flight reach the rate of a copy (65536 x

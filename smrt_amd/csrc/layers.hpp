@@ -14,10 +14,19 @@ inline int64_t max_chunks(bool ends, int64_t rows, int64_t chunk, int64_t groups
 enum Tile : int { TILE_LARGE = 0, TILE_MEDIUM = 1, TILE_SMALL = 2, TILE_ROWS = 3 };
 struct GemmPlan { int tile, chunk; };      // chunk: dW's rows a workgroup
 
-// The kernels for a few rows (layer_rows.hpp) read W once per row, so they end where their workgroups, one per row and 64 columns, are
-// two a CU for the 16-bit types and four for fp32.  1024 x 1024, row kernel | 64x64 tile, in us: bf16 1 row 6.8 | 10.8, 32 rows 8.6 | 10.8, 64 rows
-// 12.5 | 10.9; fp32 1 row 7.4 | 24.6, 32 rows 11.5 | 24.7, 64 rows 16.1 | 25.0.
-inline bool few_rows(bool f32, int64_t rows, int64_t columns) { return rows <= 64 && rows * ((columns + 63) / 64) <= (f32 ? 1024 : 512); }
+// The kernels for a few rows (layer_rows.hpp) read W once per row.  Forward they end where their workgroups, one per row and 64 columns, are two a
+// CU for the 16-bit types and five for fp32.  Row kernel | 64x64 tile, a call in us: fp32 1 x 1024 x 1024 7.4 | 24.6, 96 x 450 x 784 (1248 workgroups) 9.3 |
+// 14.2, 128 x 784 x 450 (1024) 13 | 20, 183 x 1792 x 64 7.5 | 36.8, 256 x 128 x 1024 (4096) 20.9 | 7.4; bf16 128 x 1024 x 256 (512) 7.5 | 8.1, 183 x 1792 x 64 8.3
+// | 10.9, 96 x 784 x 450 (768) 9.2 | 8.7.
+inline bool few_rows(bool f32, int64_t rows, int64_t n) { return rows * ((n + 63) / 64) <= (f32 ? 1280 : 512); }
+// Backward, where they save two launches, they take 8 us, 0.012 a workgroup of dx and 0.07 a row of a group (dW's); the tiles 17 us, 4 more for a join over groups, and
+// what dx's chain over n is longer than the other launches.  Row kernels | tiles, a call in us: fp32 66 x 64 x 64 12.5 | 17.3, 128 x 784 x 450 35 | 24, 200 x 300 x 300 36 |
+// 21, 183 x 64 x 1792 22 | 46; bf16 66 x 64 x 64 12.6 | 17.4, 183 x 64 x 1792 22 | 22.
+inline bool few_rows_backward(bool f32, int64_t rows, int64_t k, int64_t n, int64_t groups) {
+    const double own = 8.0 + 0.012 * (double)rows * (double)((k + 63) / 64) + 0.07 * (double)rows / (double)groups;
+    const double chain = (f32 ? 24.0 : 10.5) * (double)n / 1024.0 - (f32 ? 6.0 : 10.0);
+    return rows <= 256 && own <= 17.0 + (groups > 1 ? 4.0 : 0.0) + std::max(chain, 0.0);
+}
 
 // 16-bit types have 256x256 (8 waves, one workgroup a CU), 128x128 (4 or 8 waves) and 64x64 tiles whose 4 waves split the
 // summed index; fp32, whose three parts fill the registers sooner, the last two.  A launch takes its share of rounds over the 256 CUs, and at

@@ -127,7 +127,7 @@ def test_entries_refuse_null_and_small_workspaces():
     assert lib.smrt_layer_norm_backward_workspace(None) == -1
     args = _dense_args()
     assert lib.smrt_dense_backward_workspace(C.byref(args)) == 0          # a few rows have all their gradients from one launch
-    args = _dense_args(rows=100)
+    args = _dense_args(rows=300)
     need = lib.smrt_dense_backward_workspace(C.byref(args))
     assert need > 0
     assert lib.smrt_dense_backward(C.byref(args), 0xa0000, need - 1, None) == -1
@@ -166,7 +166,7 @@ def test_entries_refuse_shared_memory():
     for kw in (dict(dx=0x50000), dict(dx=0x10000), dict(dx=0x40000), dict(dw=0x20000), dict(dw=0x60000), dict(db=0x70000), dict(db=0x50000)):
         args = _dense_args(**kw)
         assert lib.smrt_dense_backward(C.byref(args), 0xa0000, 1 << 20, None) == -1 and b"overlaps" in lib.smrt_last_error(), kw
-    args = _dense_args(rows=100)
+    args = _dense_args(rows=300)
     assert lib.smrt_dense_backward(C.byref(args), 0x50000, 1 << 20, None) == -1 and b"overlaps" in lib.smrt_last_error()
     norm = dict(dtype=1, rows=4000, n=64, eps=1e-5, x=0x10000, ldx=64, weight=0x100000, y=0x200000, ldy=64, mean=0x900000, rstd=0xa00000, grad=0xb00000,
                 ldg=64, dx=0xc00000, lddx=64, dw=0xd00000, db=0xe00000)
