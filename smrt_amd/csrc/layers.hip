@@ -128,20 +128,32 @@ struct NormArgs {
     int32_t rows, n; float eps;
 };
 
-template <int TPR> struct RowSum {
-    // sum over the TPR lanes of a row; with more than a wave, all threads of the workgroup take part
-    __device__ static __forceinline__ float sum(float v, float* lds) {
+// Sums of N values over the TPR lanes of a row.  With more than a wave a row the waves' shares meet in LDS, and all threads of the workgroup take
+// part; two parts of LDS take turns, so a sum has one barrier: a part is written again only behind the next sum's, which no wave passes
+// before all have read it.
+template <int TPR, int THREADS, int N> struct RowSum {
+    static constexpr int WAVES = TPR > 64 ? TPR / 64 : 0, SLOTS = WAVES ? THREADS / 64 : 1;
+    float (*lds)[SLOTS][N];                          // [2]
+    int turn = 0;
+    __device__ __forceinline__ void operator()(float (&v)[N]) {
 #pragma unroll
-        for (int d = (TPR < 64 ? TPR : 64) / 2; d; d >>= 1) v += __shfl_xor(v, d);
-        if constexpr (TPR > 64) {
-            __syncthreads();
-            if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-            __syncthreads();
-            v = 0.0f;
+        for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int i = 0; i < TPR / 64; ++i) v += lds[i];
+            for (int d = (TPR < 64 ? TPR : 64) / 2; d; d >>= 1) v[i] += __shfl_xor(v[i], d);
+        if constexpr (WAVES > 0) {
+            const int wave = threadIdx.x >> 6, first = wave / WAVES * WAVES;
+            if ((threadIdx.x & 63) == 0)
+#pragma unroll
+                for (int i = 0; i < N; ++i) lds[turn][wave][i] = v[i];
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                v[i] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) v[i] += lds[turn][first + w][i];
+            }
+            turn ^= 1;
         }
-        return v;
     }
 };
 template <class T> __device__ __forceinline__ void load_weight(const void* p, int w_f32, int col, int valid, float fill, float (&w)[8]) {
@@ -155,7 +167,9 @@ template <class T> __device__ __forceinline__ void load_weight(const void* p, in
 template <class T, int TPR, int CH>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_forward_kernel(NormArgs p) {
     constexpr int THREADS = TPR > 256 ? TPR : 256, ROWS = THREADS / TPR;
-    __shared__ float lds[16];
+    typedef RowSum<TPR, THREADS, 1> Sum;
+    __shared__ float lds[2][Sum::SLOTS][1];
+    Sum row_sum = {lds};
     const int lane = threadIdx.x % TPR;
     float w[CH][8], b[CH][8];
 #pragma unroll
@@ -168,23 +182,25 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_forward_kernel(Nor
     for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < p.rows; row0 += (int64_t)gridDim.x * ROWS) {
         const int64_t row = row0 + threadIdx.x / TPR;
         const bool live = row < p.rows;
-        float x[CH][8], sum = 0.0f;
+        float x[CH][8], sum[1] = {};
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int col = (c * TPR + lane) * 8;
             load8f((const T*)p.x + row * p.ldx + col, live ? p.n - col : 0, x[c]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum += x[c][j];
+            for (int j = 0; j < 8; ++j) sum[0] += x[c][j];
         }
-        const float mean = RowSum<TPR>::sum(sum, lds) * inv_n;
-        float sq = 0.0f;
+        row_sum(sum);
+        const float mean = sum[0] * inv_n;
+        float sq[1] = {};
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int valid = p.n - (c * TPR + lane) * 8;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { x[c][j] -= mean; sq += j < valid ? x[c][j] * x[c][j] : 0.0f; }
+            for (int j = 0; j < 8; ++j) { x[c][j] -= mean; sq[0] += j < valid ? x[c][j] * x[c][j] : 0.0f; }
         }
-        const float rstd = 1.0f / sqrtf(RowSum<TPR>::sum(sq, lds) * inv_n + p.eps);
+        row_sum(sq);
+        const float rstd = 1.0f / sqrtf(sq[0] * inv_n + p.eps);
         if (!live) continue;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
@@ -200,15 +216,18 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_forward_kernel(Nor
 template <class T, bool PACKED, int TPR, int CH>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_backward_kernel(NormArgs p) {
     constexpr int THREADS = TPR > 256 ? TPR : 256, ROWS = THREADS / TPR;
-    __shared__ float lds[16];
-    __shared__ float sums[ROWS > 1 ? ROWS : 1][TPR <= 64 ? TPR * 8 : 1];
+    typedef RowSum<TPR, THREADS, 2> Sum;
+    __shared__ float lds[2][Sum::SLOTS][2];
+    Sum row_sum = {lds};
+    __shared__ float sums[ROWS > 1 ? ROWS : 1][ROWS > 1 ? TPR * 8 : 1];
     const int lane = threadIdx.x % TPR;
     float w[CH][8], dw[CH][8] = {}, db[CH][8] = {};
 #pragma unroll
     for (int c = 0; c < CH; ++c) { const int col = (c * TPR + lane) * 8; load_weight<T>(p.weight, p.w_f32, col, p.n - col, 1.0f, w[c]); }
     const float inv_n = 1.0f / (float)p.n;
-    // A row is requested while the one before it is worked on; with 16 waves on a row, which have no registers left for that, at its turn.
-    constexpr bool EARLY = TPR < 1024;
+    // A row is requested while the one before it is worked on; where there are no registers left for that, at its turn (32000 x 2000 bf16, four
+    // pieces a lane: 83 us, against 102 with one wave a SIMD).
+    constexpr bool EARLY = TPR < 1024 && CH < 4;
     T g_in[CH][8], x_in[PACKED ? 1 : CH][8];
     u32x2 q_in[PACKED ? CH : 1];
     uint8_t scale_in[PACKED ? CH : 1];
@@ -240,7 +259,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_backward_kernel(No
         const bool live = row < p.rows;
         if (!EARLY) request(row);
         const float mean = mean_in, rstd = rstd_in;
-        float h[CH][8], g[CH][8], s1 = 0.0f, s2 = 0.0f;
+        float h[CH][8], g[CH][8], s[2] = {};
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             if constexpr (PACKED) unpack8(q_in[c], unpack_scale(scale_in[c]), h[c]);
@@ -260,12 +279,12 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_backward_kernel(No
                 dw[c][j] += g[c][j] * h[c][j];
                 db[c][j] += g[c][j];
                 g[c][j] *= w[c][j];
-                s1 += g[c][j];
-                s2 += g[c][j] * h[c][j];
+                s[0] += g[c][j];
+                s[1] += g[c][j] * h[c][j];
             }
         }
-        s1 = RowSum<TPR>::sum(s1, lds) * inv_n;
-        s2 = RowSum<TPR>::sum(s2, lds) * inv_n;
+        row_sum(s);
+        const float s1 = s[0] * inv_n, s2 = s[1] * inv_n;
         if (!live || !p.dx) continue;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
@@ -431,20 +450,23 @@ template <class T> hipError_t launch_dz(const DzArgs& d, hipStream_t s) {
 int norm_blocks(int64_t rows, int rows_per_block, int most) { return (int)std::max<int64_t>(1, std::min<int64_t>((rows + rows_per_block - 1) / rows_per_block, most)); }
 constexpr int NORM_MAX_COLS = 1024 * 8 * 4;
 // lanes of a row and pieces of a lane, by the row's width
-template <class F> hipError_t by_width(int64_t n, F f) {
+template <bool BACKWARD, class F> hipError_t by_width(int64_t n, F f) {
     if (n <= 64) return f(std::integral_constant<int, 8>(), std::integral_constant<int, 1>());
     if (n <= 128) return f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
     if (n <= 256) return f(std::integral_constant<int, 32>(), std::integral_constant<int, 1>());
     if (n <= 512) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
     if (n <= 1024) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+    // a wave a row as far as registers go, then two: more waves wait for each other at every row (46700 x 1437 bf16 backward 262 us with four
+    // waves a row, 109 with one)
     if (n <= 1536) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 3>());
     if (n <= 2048) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
-    if (n <= 4096) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
+    // (20000 x 2500 bf16, two waves a row | four: backward 92 | 122 us, forward, which keeps no sums, 50 | 45)
+    if (n <= 4096) return f(std::integral_constant<int, BACKWARD ? 128 : 256>(), std::integral_constant<int, BACKWARD ? 4 : 2>());
     if (n <= 8192) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
     if (n <= 16384) return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
     return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
 }
-int norm_rows_per_block(int64_t n) { return n <= 64 ? 32 : n <= 128 ? 16 : n <= 256 ? 8 : n <= 2048 ? 4 : 1; }
+int norm_rows_per_block(int64_t n) { return n <= 64 ? 32 : n <= 128 ? 16 : n <= 256 ? 8 : n <= 2048 ? 4 : n <= 4096 ? 2 : 1; }      // of the backward pass
 // Workgroups of the forward pass: four turns each, so that weight and bias are read once for them, where that leaves eight a CU
 int norm_forward_blocks(int64_t rows, int per) { return std::max(norm_blocks(rows, per, 2048), norm_blocks(rows, 4 * per, 4096)); }
 // Workgroups of the backward pass: four turns each up to two a CU, which with the next row in flight reach the rate of a copy (65536 x
@@ -626,7 +648,7 @@ extern "C" int smrt_layer_norm_forward(const smrt_layer_norm* p, void* hip_strea
         return fail(who, "an output overlaps a weight or another output");
     const NormArgs a = norm_args(p);
     return launched(who, by_type(p->dtype, [&](auto t) {
-        return by_width(p->n, [&](auto tpr, auto ch) {
+        return by_width<false>(p->n, [&](auto tpr, auto ch) {
             constexpr int TPR = decltype(tpr)::value, THREADS = TPR > 256 ? TPR : 256;
             hipLaunchKernelGGL((norm_forward_kernel<decltype(t), TPR, decltype(ch)::value>), dim3(norm_forward_blocks(p->rows, THREADS / TPR)), dim3(THREADS), 0,
                                (hipStream_t)hip_stream, a);
@@ -660,7 +682,7 @@ extern "C" int smrt_layer_norm_backward(const smrt_layer_norm* p, void* workspac
     const int blocks = norm_backward_blocks(p->rows, p->n);
     a.part = need ? (float*)workspace : nullptr;
     hipError_t e = by_type(p->dtype, [&](auto t) {
-        return by_width(p->n, [&](auto tpr, auto ch) {
+        return by_width<true>(p->n, [&](auto tpr, auto ch) {
             constexpr int TPR = decltype(tpr)::value, CH = decltype(ch)::value, THREADS = TPR > 256 ? TPR : 256;
             if (p->x_scale) hipLaunchKernelGGL((norm_backward_kernel<decltype(t), true, TPR, CH>), dim3(blocks), dim3(THREADS), 0, stream, a);
             else hipLaunchKernelGGL((norm_backward_kernel<decltype(t), false, TPR, CH>), dim3(blocks), dim3(THREADS), 0, stream, a);
