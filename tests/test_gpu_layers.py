@@ -920,3 +920,15 @@ def test_class_decoders_without_rows(fitted):
     assert d.generate([0, 0, 0], np.random.RandomState(1)).shape == (0, 50)
     some = d.generate([0, 4, 0], np.random.RandomState(1))
     assert torch.equal(some, ClassDecoders(fitted[1:2]).generate([4], np.random.RandomState(1)))
+
+
+WIDE_NORMS = [(2051, 1437), (2050, 2000), (1031, 2500), (1029, 4000), (1025, 8000), (517, 12000)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("i", range(len(WIDE_NORMS)), ids=[str(s) for s in WIDE_NORMS])
+def test_layer_norm_of_many_wide_rows(i, dtype, monkeypatch):
+    """Every way to share a row among waves, with more rows than one turn of the workgroups and odd numbers of them."""
+    import sys
+    monkeypatch.setattr(sys.modules[__name__], "NORMS", WIDE_NORMS)
+    test_layer_norm(i, dtype)
