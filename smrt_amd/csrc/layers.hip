@@ -538,7 +538,7 @@ extern "C" int smrt_dense_forward(const smrt_dense* p, void* hip_stream) {
     else if (p->a) { g.act_out = p->a; g.ld_act = p->lda; }
     g.ends = p->ends; g.groups = p->groups; g.keep_rest = p->keep_rest; g.rows = (int32_t)p->rows;
     g.M = (int32_t)p->rows; g.N = (int32_t)p->n; g.K = (int32_t)p->k; g.act = p->activation;
-    return launched(who, gemm(p->dtype, LAYOUT_FORWARD, plan_gemm(LAYOUT_FORWARD, p->dtype == SMRT_F32, p->rows, p->rows, p->n, p->groups), g, (hipStream_t)hip_stream));
+    return launched(who, gemm(p->dtype, LAYOUT_FORWARD, plan_gemm(LAYOUT_FORWARD, p->dtype == SMRT_F32, p->rows, p->rows, p->n, p->groups, p->k, g.q_out != nullptr), g, (hipStream_t)hip_stream));
 }
 
 extern "C" int64_t smrt_dense_backward_workspace(const smrt_dense* p) {

@@ -35,7 +35,10 @@ inline bool few_rows_backward(bool f32, int64_t rows, int64_t k, int64_t n, int6
 //             fp32:                        128x128  54   | 45       64x64  24   | 15.5
 // so 65536 x 1024 x 1024 in bf16 took 152 / 155 / 269 us on the three, 4096 x 1024 x 1024 35 / 21 / 25, 40000 x 784 x 450 61 / 51 / 90,
 // 1024 x 784 x 450 28 / 19 / 12; in fp32 65536 x 1024 x 1024 702 / 976 us on the two, 1024 x 784 x 450 48 / 25.
-inline GemmPlan plan_gemm(int layout, bool f32, int64_t rows, int64_t m, int64_t n, int64_t groups) {
+// The forward epilogue of the 256x256 tile has nothing beside it on its CU: 6 us a round, 9 with the 8-bit form (bf16, 256x256 | 128x128: 32768 x 256 x 1024 relu
+// 40 | 33 us, 65536 x 512 x 1024 sigmoid 108 | 95, 32768 x 1024 x 1024 elu in 8 bits 104 | 99, 65536 x 2000 x 1024 relu 282 | 325).
+// k: forward, the summed index.
+inline GemmPlan plan_gemm(int layout, bool f32, int64_t rows, int64_t m, int64_t n, int64_t groups, int64_t k = 0, bool packed = false) {
     constexpr int side[3] = {256, 128, 64};
     constexpr double chain[2][3] = {{30, 17, 10.5}, {1e9, 54, 24}}, round[2][3] = {{40, 11.7, 5.6}, {1e9, 45, 15.5}};
     if (layout == LAYOUT_FORWARD && few_rows(f32, rows, n)) return {TILE_ROWS, 0};
@@ -61,7 +64,8 @@ inline GemmPlan plan_gemm(int layout, bool f32, int64_t rows, int64_t m, int64_t
             us += 2.0 * (double)max_slabs(rows, chunk, groups) * m * n * 4.0 / 5e6;
         } else {
             const int64_t tiles = (groups == 1 ? (rows + side[t] - 1) / side[t] : rows / side[t] + groups / 2) * tn;     // about half a tile a group is empty
-            us = std::max(chain[f32][t], round[f32][t] * (double)((tiles + 255) / 256));
+            const double epilogue = layout == LAYOUT_FORWARD && t == TILE_LARGE ? (packed ? 9.0 : 6.0) * 1024.0 / (double)std::max<int64_t>(k, 1) : 0.0;
+            us = std::max(chain[f32][t], round[f32][t] * (double)((tiles + 255) / 256)) + epilogue * (double)((tiles + 255) / 256);
         }
         if (us < best_us) { best_us = us; best = p; }
     }
