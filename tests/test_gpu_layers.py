@@ -932,3 +932,20 @@ def test_layer_norm_of_many_wide_rows(i, dtype, monkeypatch):
     import sys
     monkeypatch.setattr(sys.modules[__name__], "NORMS", WIDE_NORMS)
     test_layer_norm(i, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("k", [1, 7, 9, 33, 65, 72, 129, 135])
+def test_every_way_a_piece_is_cut_with_many_rows(k, dtype):
+    """The same widths forward with more rows than the kernels for a few rows take, bias, residual and the saved activation among them."""
+    from smrt_amd.autoencode import dense, pack_rows
+    rng = np.random.default_rng(7500 + k)
+    m = 1301
+    x = make(rng, dtype, m, k)
+    for n in WIDTHS:
+        w, b, r = make(rng, dtype, k, n, scale=k ** -0.5), make(rng, dtype, n), make(rng, dtype, m, n)
+        y, saved = dense(odd_rows(x), odd_rows(w), b.cuda(), residual=odd_rows(r), activation="tanh", save="activation")
+        check_dense(x, w, b, r, "tanh", y, saved, dtype)
+        y8, kept = dense(odd_rows(x), odd_rows(w), b.cuda(), residual=odd_rows(r), activation="tanh", save="packed")
+        want = pack_rows(saved)
+        assert torch.equal(y8, y) and torch.equal(kept.q, want.q) and torch.equal(kept.scale, want.scale)
