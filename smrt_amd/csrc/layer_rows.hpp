@@ -78,7 +78,7 @@ struct RowsBackward {
     const void* x; int64_t ldx; const uint8_t* x_scale; int64_t ld_x_scale;
     const void* w; int64_t ldw, w_stride;
     void* dx; int64_t lddx; void* dw; int64_t lddw, dw_stride; void* db; int64_t db_stride;      // each may be null
-    const int64_t* ends; int32_t groups, rows, k, n, act;
+    const int64_t* ends; int32_t groups, keep_rest, rows, k, n, act;     // keep_rest: dx of rows of no group stays as it is
     int32_t tiles_k, tiles_n, dx_blocks;            // of 64; dx_blocks = rows * tiles_k, or 0 without dx
 };
 
@@ -117,6 +117,7 @@ template <class T> __global__ void __launch_bounds__(ROWS_THREADS, 2) rows_backw
         const int row = bid / p.tiles_k, k0 = (bid % p.tiles_k) * 64 + wave * 8;
         int group = 0;
         if (p.ends) group = __builtin_amdgcn_readfirstlane(row_group(p.ends, p.groups, p.rows, row));
+        if (group < 0 && p.keep_rest) return;
         const T* const w = (const T*)p.w + (int64_t)(group < 0 ? 0 : group) * p.w_stride;
         float acc[8] = {};
         for (int n0 = 0; n0 < (group < 0 ? 0 : p.n); n0 += 512) {

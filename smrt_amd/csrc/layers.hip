@@ -575,7 +575,7 @@ extern "C" int smrt_dense_backward(const smrt_dense* p, void* workspace, int64_t
         r.grad = p->grad; r.ldg = p->ldg; r.a = p->a; r.lda = p->lda; r.a_scale = p->a_scale; r.ld_a_scale = p->ld_a_scale;
         r.x = p->x; r.ldx = p->ldx; r.x_scale = p->x_scale; r.ld_x_scale = p->ld_x_scale; r.w = p->w; r.ldw = p->ldw; r.w_stride = p->w_stride;
         r.dx = p->k ? p->dx : nullptr; r.lddx = p->lddx; r.dw = p->k ? p->dw : nullptr; r.lddw = p->lddw; r.dw_stride = p->dw_stride; r.db = p->db; r.db_stride = p->bias_stride;
-        r.ends = p->ends; r.groups = p->groups; r.rows = (int32_t)p->rows; r.k = (int32_t)p->k; r.n = (int32_t)p->n; r.act = p->activation;
+        r.ends = p->ends; r.groups = p->groups; r.keep_rest = p->keep_rest; r.rows = (int32_t)p->rows; r.k = (int32_t)p->k; r.n = (int32_t)p->n; r.act = p->activation;
         const int32_t tiles_k = (int32_t)((p->k + 63) / 64);
         r.dx_blocks = r.dx ? r.rows * tiles_k : 0;
         r.tiles_k = r.dw || r.dx ? tiles_k : 1;

@@ -949,3 +949,34 @@ def test_every_way_a_piece_is_cut_with_many_rows(k, dtype):
         y8, kept = dense(odd_rows(x), odd_rows(w), b.cuda(), residual=odd_rows(r), activation="tanh", save="packed")
         want = pack_rows(saved)
         assert torch.equal(y8, y) and torch.equal(kept.q, want.q) and torch.equal(kept.scale, want.scale)
+
+
+# ------------------------------------------------------------------------------------------------ what a C caller may ask for besides
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("m,k,n,ends,act", [(40, 90, 70, [7, 7, 31], "elu"), (12, 33, 130, [0, 5], "identity"), (300, 90, 70, [100, 90, 221], "sigmoid"),
+                                            (700, 90, 70, [100, 301, 333], "tanh"), (9000, 300, 520, [4000, 8001], "identity"),
+                                            (40, 90, 70, [0, 0], "relu"), (700, 90, 70, [0, 0], "relu")])
+def test_backward_entry_keeps_rows_of_no_class(m, k, n, ends, act, dtype):
+    """keep_rest of the C entry: dx of rows behind the last end stays as it was, from the kernels for a few rows and from the product tiles alike."""
+    import ctypes as C
+    from smrt_amd import _hip
+    from smrt_amd.autoencode import dense_grouped, dense_grouped_backward
+    rng = np.random.default_rng(900)
+    G, ids = len(ends), {F32: 0, BF16: 1, F16: 2}
+    x, w, g = make(rng, dtype, m, k).cuda(), make(rng, dtype, G, k, n, scale=k ** -0.5).cuda(), make(rng, dtype, m, n).cuda()
+    e = torch.tensor(ends, device="cuda")
+    saved = dense_grouped(x, e, w, activation=act, save="activation")[1]
+    want = dense_grouped_backward(g, x, e, w, saved, activation=act)
+    lib = _hip.load()
+    for keep in (1, 0):
+        dx, dw, db = torch.full((m, k), 5.0, dtype=dtype, device="cuda"), torch.empty_like(w), torch.empty((G, n), dtype=dtype, device="cuda")
+        args = _hip.Dense(ids[dtype], _hip.ACTIVATION_IDS[act], m, k, n, G, keep, e.data_ptr(), x.data_ptr(), k, None, 0, w.data_ptr(), n, k * n, None, n,
+                          None, 0, None, 0, None if saved is None else saved.data_ptr(), n, None, 0, g.data_ptr(), n, dx.data_ptr(), k, dw.data_ptr(), n, k * n,
+                          db.data_ptr())
+        size = lib.smrt_dense_backward_workspace(C.byref(args))
+        assert (size > 0) == (m >= 300)
+        work = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda")
+        assert lib.smrt_dense_backward(C.byref(args), work.data_ptr(), size, torch.cuda.current_stream().cuda_stream) == 0
+        last = max(ends)
+        assert torch.equal(dx[:last], want[0][:last]) and torch.equal(dw, want[1]) and torch.equal(db, want[2])
+        assert (dx[last:] == (5.0 if keep else 0.0)).all()
