@@ -980,3 +980,98 @@ def test_backward_entry_keeps_rows_of_no_class(m, k, n, ends, act, dtype):
         last = max(ends)
         assert torch.equal(dx[:last], want[0][:last]) and torch.equal(dw, want[1]) and torch.equal(db, want[2])
         assert (dx[last:] == (5.0 if keep else 0.0)).all()
+
+
+TILED = [(1408, 70, 50), (1500, 9, 450), (16500, 70, 700), (70000, 40, 260)]       # 64x64 tiles, the same, 128x128 and, in 16 bits, 256x256
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", [(40, 70, 50)] + TILED)
+def test_infinities_and_nan_from_rows_and_tiles(m, k, n, dtype):
+    """Infinities keep their sign and NaN its place in all three products, whichever kernel takes them."""
+    from smrt_amd.autoencode import dense, dense_backward
+    rng = np.random.default_rng(920)
+    inf, nan, top = float("inf"), float("nan"), torch.finfo(dtype).max
+    x, w, g = make(rng, dtype, m, k), make(rng, dtype, k, n), make(rng, dtype, m, n)
+    x[3, 5], x[7, k - 1], x[11, 0], x[12, 1], x[m - 1, k - 1] = inf, -inf, nan, top, inf
+    w[2, 9], w[4, 11], w[k - 1, n - 1] = inf, 0.0, -inf
+    g[20, 3], g[21, n - 1], g[m - 2, 0], g[23, 7] = inf, -inf, nan, top
+
+    def doubtful(a, b):
+        """What 32-bit sums may take elsewhere: results near the largest number of the type, and sums in which a term of the largest number and a factor
+        above 1, an infinity in 32 bits (not in f16, whose products stay far below), meets an infinity or another such term."""
+        want, has = a @ b, lambda f, d: f.any(d)
+        big = want.isfinite() & (want.abs() > 0.9 * top)
+        if dtype != F16:
+            huge = lambda v: (v.abs() == top) | v.isinf()
+            big |= has(a.abs() == top, 1)[:, None] & has(huge(b), 0) | has(huge(a), 1)[:, None] & has(b.abs() == top, 0)
+        return big
+
+    def check(got, a, b, what):
+        got, want, big = got.cpu().double(), a @ b, doubtful(a, b)
+        for f in (torch.isnan, torch.isposinf, torch.isneginf):
+            assert torch.equal(f(got)[~big], f(want)[~big]), (what, f.__name__)
+        assert want.isposinf().any() and want.isneginf().any() and want.isnan().any() and want.isfinite().any()
+    X, W, D = x.double(), w.double(), g.double()
+    check(dense(x.cuda(), w.cuda()), X, W, "y")
+    dx, dw, db = dense_backward(g.cuda(), x.cuda(), w.cuda())
+    check(dx, D, W.T, "dx")
+    check(dw, X.T, D, "dw")
+    check(db[None], torch.ones(1, m, dtype=torch.float64), D, "db")
+    nans, sure = (X @ W).isnan(), ~doubtful(X, W)
+    for act in ACTS:
+        assert torch.equal(dense(x.cuda(), w.cuda(), activation=act).cpu().isnan()[sure], nans[sure]), act
+
+
+@pytest.mark.parametrize("m,k,n", TILED)
+def test_small_and_large_numbers_from_tiles(m, k, n):
+    """fp32 in parts over the range in which all three parts are normal numbers (x from 2^-103, so that x's last bit is 2^-126), and near the largest."""
+    from smrt_amd.autoencode import dense, dense_backward
+    rng = np.random.default_rng(930)
+    x, w, g = make(rng, F32, m, k).clamp(-3, 3), make(rng, F32, k, n, scale=k ** -0.5), make(rng, F32, m, n).clamp(-3, 3)
+    X, W, D = x.double(), w.double(), g.double()
+    for s in (2.0 ** -100, 2.0 ** 110):
+        y = dense((x * s).cuda(), w.cuda()).cpu().double() / s
+        assert (y - X @ W).norm() <= 2e-6 * (X @ W).norm()
+        dx, dw, _ = dense_backward((g * s).cuda(), x.cuda(), w.cuda())
+        assert (dx.cpu().double() / s - D @ W.T).norm() <= 2e-6 * (D @ W.T).norm()
+        assert (dw.cpu().double() / s - X.T @ D).norm() <= 2e-6 * (X.T @ D).norm()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("m,ends,k,n", [(1500, [300, 701, 1400], 70, 45), (17000, [5000, 9001, 16800], 70, 700)])
+def test_nan_stays_in_its_class_in_tiles(m, ends, k, n, dtype):
+    """A class of NaN rows, NaN rows of no class and a NaN weight leave the other classes' results as they are."""
+    from smrt_amd.autoencode import dense_grouped, dense_grouped_backward
+    rng = np.random.default_rng(940)
+    nan = float("nan")
+    x, w, g = make(rng, dtype, m, k), make(rng, dtype, 3, k, n, scale=0.1), make(rng, dtype, m, n)
+    e = torch.tensor(ends, device="cuda")
+
+    def run(x, w, g):
+        y, saved = dense_grouped(x.cuda(), e, w.cuda(), activation="sigmoid", save="activation")
+        return (y, *dense_grouped_backward(g.cuda(), x.cuda(), e, w.cuda(), saved, activation="sigmoid"))
+    want = run(x, w, g)
+    x, w, g = x.clone(), w.clone(), g.clone()
+    x[ends[0]:ends[1]] = nan
+    x[ends[2]:], g[ends[2]:] = nan, nan
+    y, dx, dw, db = run(x, w, g)
+    a, b, c = slice(0, ends[0]), slice(ends[0], ends[1]), slice(ends[1], ends[2])
+    for s in (a, c):
+        assert torch.equal(y[s], want[0][s]) and torch.equal(dx[s], want[1][s])
+    assert y[b].isnan().all() and dx[b].isnan().all() and dw[1].isnan().all() and db[1].isnan().all()
+    for j in (0, 2):
+        assert torch.equal(dw[j], want[2][j]) and torch.equal(db[j], want[3][j])
+    assert not y[ends[2]:].any() and not dx[ends[2]:].any()
+    w[2, 5, 7] = nan
+    y = run(x, w, g)[0]
+    assert torch.equal(y[a], want[0][a]) and y[c, 7].isnan().all() and torch.equal(y[c, :7], want[0][c, :7]) and torch.equal(y[c, 8:], want[0][c, 8:])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", TILED)
+def test_grouped_tiles_are_dense_tiles_for_one_group(m, k, n, dtype):
+    from smrt_amd.autoencode import dense, dense_grouped
+    rng = np.random.default_rng(950)
+    x, w = make(rng, dtype, m, k).cuda(), make(rng, dtype, k, n).cuda()
+    assert torch.equal(dense_grouped(x, torch.tensor([m], device="cuda"), w[None]), dense(x, w))
