@@ -189,3 +189,29 @@ def test_class_decoders_refuse():
         ClassDecoders([VariationalAutoEncoder(4, 2)], dtype=torch.float64)
     with pytest.raises(NotFittedError):
         ClassDecoders([VariationalAutoEncoder(4, 2)])
+
+
+def test_the_package_is_imported_without_torch():
+    """Only the layers need torch; asking for one of their names brings it in."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys
+import smrt_amd.autoencode as a, smrt_amd.balance, smrt_amd.utils
+assert "torch" not in sys.modules
+names = ["ClassDecoders", "PackedRows", "class_decoders", "dense", "dense_backward", "dense_grouped", "dense_grouped_backward", "layer_norm",
+         "layer_norm_backward", "layers", "pack_rows", "unpack_rows"]
+assert set(names) <= set(a.__all__) and set(names) <= set(dir(a)) and "torch" not in sys.modules
+assert a.dense is a.layers.dense and a.ClassDecoders is a.class_decoders.ClassDecoders and "torch" in sys.modules
+assert sorted(set(a.layers.__all__ + a.class_decoders.__all__ + ["layers", "class_decoders"])) == sorted(names)
+try:
+    a.no_such_name
+except AttributeError as e:
+    assert "no_such_name" in str(e)
+else:
+    raise AssertionError
+from smrt_amd.autoencode import *
+assert layer_norm is a.layer_norm and VariationalAutoEncoder is a.VariationalAutoEncoder
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
