@@ -382,6 +382,14 @@ Span weights(const void* p, int64_t groups, int64_t stride, int64_t k, int64_t l
     return groups == 1 ? matrix(p, k, ld, n, es) : piece(p, ((groups - 1) * stride + span(k, ld, n)) * es);
 }
 
+// scale bytes of an 8-bit form (null: the matrix is not in 8 bits)
+Span scales(const uint8_t* p, int64_t rows, int64_t ld, int64_t n) { return matrix(p, rows, ld, (n + PACK_BLOCK - 1) / PACK_BLOCK, 1); }
+// a matrix that an earlier pass kept, of dtype or in 8 bits
+Span kept(const void* p, const uint8_t* scale, int64_t rows, int64_t ld, int64_t n, int64_t es) {
+    return scale ? matrix(p, rows, ld, pad(n, PACK_BLOCK), 1) : matrix(p, rows, ld, n, es);
+}
+Span ends_of(const smrt_dense* p) { return piece(p->ends, p->groups * 8); }
+
 int check_dense(const smrt_dense* p, const char* who) {
     if (!p) return fail(who, "null argument");
     if (p->dtype < 0 || p->dtype > SMRT_F16) return fail(who, "dtype must be SMRT_F32, SMRT_BF16 or SMRT_F16");
@@ -500,7 +508,7 @@ int check_pack(const char* who, int dtype, const void* x, int64_t ldx, int64_t r
     if (rows < 0 || rows > MAX_ROWS || n < 0 || n > MAX_COLS) return fail(who, "bad sizes");
     if (ldx < n || ldq < pad(n, PACK_BLOCK) || ld_scale < (n + PACK_BLOCK - 1) / PACK_BLOCK) return fail(who, "a leading dimension is below its columns");
     if (rows && n && (!x || !q || !scale)) return fail(who, "null pointer");
-    if (any_overlap({matrix(x, rows, ldx, n, elem_size(dtype)), matrix(q, rows, ldq, pad(n, PACK_BLOCK), 1), matrix(scale, rows, ld_scale, (n + PACK_BLOCK - 1) / PACK_BLOCK, 1)}, {}))
+    if (any_overlap({matrix(x, rows, ldx, n, elem_size(dtype)), matrix(q, rows, ldq, pad(n, PACK_BLOCK), 1), scales((const uint8_t*)scale, rows, ld_scale, n)}, {}))
         return fail(who, "the matrix and its 8-bit form overlap");
     return 0;
 }
@@ -523,13 +531,12 @@ extern "C" int smrt_dense_forward(const smrt_dense* p, void* hip_stream) {
     if (p->rows == 0 || p->n == 0) return 0;
     if (!p->y) return fail(who, "null pointer");
     const int64_t es = elem_size(p->dtype);
-    const int64_t blocks = (p->n + PACK_BLOCK - 1) / PACK_BLOCK;
     const Span y = matrix(p->y, p->rows, p->ldy, p->n, es), residual = matrix(p->residual, p->rows, p->ldr, p->n, es);
-    const Span a = p->a_scale ? matrix(p->a, p->rows, p->lda, blocks * PACK_BLOCK, 1) : matrix(p->a, p->rows, p->lda, p->n, es);
+    const Span a = kept(p->a, p->a_scale, p->rows, p->lda, p->n, es), a_scale = scales(p->a ? p->a_scale : nullptr, p->rows, p->ld_a_scale, p->n);
+    const Span bias = p->groups == 1 ? piece(p->bias, p->n * es) : matrix(p->bias, p->groups, p->bias_stride, p->n, es);
     const bool in_place = p->residual == p->y && p->ldr == p->ldy;
-    if (any_overlap({y, a, matrix(p->a ? p->a_scale : nullptr, p->rows, p->ld_a_scale, blocks, 1)},
-                    {matrix(p->x, p->rows, p->ldx, p->k, es), weights(p->w, p->groups, p->w_stride, p->k, p->ldw, p->n, es), in_place ? Span{} : residual}) ||
-        overlap(a, residual))
+    if (any_overlap({y, a, a_scale}, {matrix(p->x, p->rows, p->ldx, p->k, es), weights(p->w, p->groups, p->w_stride, p->k, p->ldw, p->n, es), bias, ends_of(p),
+                                      in_place ? Span{} : residual}))
         return fail(who, "an output overlaps an input or another output (y may only be the residual itself)");
     GemmArgs g = {};
     g.A = p->x; g.lda = p->ldx; g.B = p->w; g.ldb = p->ldw; g.strideB = p->w_stride; g.C = p->y; g.ldc = p->ldy;
@@ -566,8 +573,9 @@ extern "C" int smrt_dense_backward(const smrt_dense* p, void* workspace, int64_t
     const bool reads_a = p->activation != SMRT_ACT_IDENTITY;
     if (any_overlap({matrix(p->dx, p->rows, p->lddx, p->k, es), weights(p->dw, p->groups, p->dw_stride, p->k, p->lddw, p->n, es),
                      piece(p->db, ((p->groups - 1) * p->bias_stride + p->n) * es), piece(workspace, b.total)},
-                    {matrix(p->grad, p->rows, p->ldg, p->n, es), weights(p->w, p->groups, p->w_stride, p->k, p->ldw, p->n, es),
-                     matrix(p->x, p->rows, p->ldx, p->k, p->x_scale ? 1 : es), matrix(reads_a ? p->a : nullptr, p->rows, p->lda, p->n, packed_a ? 1 : es)}))
+                    {matrix(p->grad, p->rows, p->ldg, p->n, es), weights(p->w, p->groups, p->w_stride, p->k, p->ldw, p->n, es), ends_of(p),
+                     kept(p->x, p->x_scale, p->rows, p->ldx, p->k, es), scales(p->x_scale, p->rows, p->ld_x_scale, p->k),
+                     kept(reads_a ? p->a : nullptr, p->a_scale, p->rows, p->lda, p->n, es), scales(reads_a ? p->a_scale : nullptr, p->rows, p->ld_a_scale, p->n)}))
         return fail(who, "an output or the workspace overlaps an input or another output");
     if (b.total > workspace_bytes || (b.total && !workspace)) return fail(who, "the workspace is smaller than smrt_dense_backward_workspace says");
     if (b.rows) {
@@ -641,11 +649,13 @@ extern "C" int smrt_layer_norm_forward(const smrt_layer_norm* p, void* hip_strea
     if (!p->y) return fail(who, "null pointer");
     if (!(p->eps >= 0.0f)) return fail(who, "eps must be >= 0");
     const int64_t es = elem_size(p->dtype);
-    if ((p->x != p->y || p->ldx != p->ldy) && overlap(matrix(p->y, p->rows, p->ldy, p->n, es), matrix(p->x, p->rows, p->ldx, p->n, es)))
+    const Span x = matrix(p->x, p->rows, p->ldx, p->n, es);
+    if ((p->x != p->y || p->ldx != p->ldy) && overlap(matrix(p->y, p->rows, p->ldy, p->n, es), x))
         return fail(who, "y overlaps x (it may only be x itself)");
     const int64_t ws = p->n * (p->weight_f32 ? 4 : es);
-    if (any_overlap({matrix(p->y, p->rows, p->ldy, p->n, es), piece(p->mean, p->rows * 4), piece(p->rstd, p->rows * 4)}, {piece(p->weight, ws), piece(p->bias, ws)}))
-        return fail(who, "an output overlaps a weight or another output");
+    const Span mean = piece(p->mean, p->rows * 4), rstd = piece(p->rstd, p->rows * 4);
+    if (any_overlap({matrix(p->y, p->rows, p->ldy, p->n, es), mean, rstd}, {piece(p->weight, ws), piece(p->bias, ws)}) || any_overlap({mean, rstd}, {x}))
+        return fail(who, "an output overlaps an input or another output");
     const NormArgs a = norm_args(p);
     return launched(who, by_type(p->dtype, [&](auto t) {
         return by_width<false>(p->n, [&](auto tpr, auto ch) {
@@ -674,7 +684,7 @@ extern "C" int smrt_layer_norm_backward(const smrt_layer_norm* p, void* workspac
     const int64_t need = smrt_layer_norm_backward_workspace(p);
     const int64_t es = elem_size(p->dtype), ws = p->n * (p->weight_f32 ? 4 : es);
     if (any_overlap({matrix(p->dx, p->rows, p->lddx, p->n, es), piece(p->dw, ws), piece(p->db, ws), piece(workspace, need)},
-                    {matrix(p->grad, p->rows, p->ldg, p->n, es), matrix(p->x, p->rows, p->ldx, p->n, p->x_scale ? 1 : es), piece(p->weight, ws),
+                    {matrix(p->grad, p->rows, p->ldg, p->n, es), kept(p->x, p->x_scale, p->rows, p->ldx, p->n, es), scales(p->x_scale, p->rows, p->ld_x_scale, p->n), piece(p->weight, ws),
                      piece(p->mean, p->rows * 4), piece(p->rstd, p->rows * 4)}))
         return fail(who, "an output or the workspace overlaps an input or another output");
     if (need > workspace_bytes || (need && !workspace)) return fail(who, "the workspace is smaller than smrt_layer_norm_backward_workspace says");

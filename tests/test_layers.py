@@ -215,3 +215,31 @@ from smrt_amd.autoencode import *
 assert layer_norm is a.layer_norm and VariationalAutoEncoder is a.VariationalAutoEncoder
 """
     subprocess.run([sys.executable, "-c", code], check=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+
+def test_entries_refuse_outputs_over_any_input():
+    """Biases, ends, scale bytes and a norm's input count as much as the matrices do."""
+    lib = _hip.load()
+
+    def refused(fn, args, *rest):
+        assert fn(C.byref(args), *rest, None) == -1 and b"overlaps" in lib.smrt_last_error(), args
+    groups = dict(rows=40, groups=2, ends=0x200000, w_stride=128)
+    for kw in (dict(bias=0x30010), dict(bias=0x40010), dict(bias=0x2fffc), dict(bias=0x30000, residual=0x30000, ldr=16),
+               dict(groups, bias=0x30100, bias_stride=16), dict(groups, bias=0x2ff80, bias_stride=40), dict(groups, ends=0x30010), dict(groups, ends=0x2fff8),
+               dict(groups, ends=0x3fff8), dict(rows=4, ends=0x30000),
+               dict(a_scale=0x90000, lda=32, ld_a_scale=1, bias=0x8fff0), dict(a_scale=0x90000, lda=32, ld_a_scale=1, residual=0x90000, ldr=16),
+               dict(groups, a_scale=0x90000, lda=32, ld_a_scale=1, ends=0x8fff8)):
+        refused(lib.smrt_dense_forward, _dense_args(**kw))
+    packed_x, packed_a = dict(x_scale=0x90000, ldx=32, ld_x_scale=1), dict(a_scale=0x98000, lda=32, ld_a_scale=1)
+    for kw in (dict(groups, dx=0x200008), dict(groups, db=0x1ffffc), dict(groups, dw=0x1fff00), dict(rows=4, ends=0x60000),
+               dict(packed_x, dx=0x90000), dict(packed_x, dw=0x8ff00), dict(packed_x, db=0x90000), dict(packed_a, dx=0x98000), dict(packed_a, db=0x97ffc),
+               dict(packed_x, db=0x10008)):
+        refused(lib.smrt_dense_backward, _dense_args(**kw), 0xa0000, 1 << 20)
+    refused(lib.smrt_dense_backward, _dense_args(rows=300, a_scale=0xa0010, lda=32, ld_a_scale=1), 0xa0000, 1 << 20)
+    refused(lib.smrt_dense_backward, _dense_args(rows=300, groups=2, ends=0xa0100, w_stride=128), 0xa0000, 1 << 20)
+    norm = dict(dtype=1, rows=4000, n=64, eps=1e-5, x=0x10000, ldx=64, weight=0x100000, y=0x200000, ldy=64, mean=0x900000, rstd=0xa00000, grad=0xb00000,
+                ldg=64, dx=0xc00000, lddx=64, dw=0xd00000, db=0xe00000)
+    for kw in (dict(mean=0x10000), dict(rstd=0x12000), dict(y=0x10000, mean=0x10000)):
+        refused(lib.smrt_layer_norm_forward, _hip.LayerNorm(**{**norm, **kw}))
+    for kw in (dict(x_scale=0xd00000, ld_x_scale=2), dict(x_scale=0xcffff0, ld_x_scale=2, dx=None), dict(x=0xd00000 - 3999 * 96 - 48, ldx=96, n=40, x_scale=0x80000, ld_x_scale=2)):
+        refused(lib.smrt_layer_norm_backward, _hip.LayerNorm(**{**norm, **kw}), 0x2000000, 1 << 30)
