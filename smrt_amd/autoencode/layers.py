@@ -13,13 +13,14 @@ graph (smrt/autoencode/layer.py:348-464).
 Tensors are ``float32``, ``bfloat16`` or ``float16`` on one GPU, 2-d, with a row's elements next to each other (rows may
 be any distance apart); sums are fp32.  Work is queued on the device's current torch stream and nothing waits for it, so the calls
 can be captured into graphs.  They take no part in torch's autograd -- the gradients are calls of their own -- and
-refuse a tensor that requires grad while grad mode is on.  There is no CPU fallback.
+refuse a tensor that requires grad while grad mode is on, or that has a tangent.  There is no CPU fallback.
 """
 from __future__ import annotations
 
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _hip
 
@@ -32,10 +33,11 @@ _BLOCK = 32                                      # columns that share a scale by
 
 
 # A small layer is over in a few microseconds, so the checks have a short way for the usual argument -- a plain tensor of the
-# right type, device and layout -- and words only for the others.
+# right type, device and layout, outside of every level of forward-mode differentiation (number -1) -- and words only for the others.
 def _tensor(t, name, dim, dtype, dev):
     """Checks any tensor argument; ``dtype`` None: one of the three types, ``dev`` None: any device."""
-    if type(t) is _Tensor and t.dtype is dtype and t.get_device() == dev and not t.requires_grad and t.is_contiguous() and t.dim() == dim:
+    if type(t) is _Tensor and t.dtype is dtype and t.get_device() == dev and not t.requires_grad and t.is_contiguous() and t.dim() == dim \
+            and forward_ad._current_level < 0:
         return t
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a torch tensor, got %s" % (name, type(t).__name__))
@@ -50,6 +52,8 @@ def _tensor(t, name, dim, dtype, dev):
         raise ValueError("%s is on %s, expected %s" % (name, t.device, "the CPU" if dev < 0 else "cuda:%d" % dev))
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError("%s requires grad, and the layer calls take no part in autograd: detach it, or call under torch.no_grad()" % name)
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError("%s has a tangent, and the layer calls take no part in autograd: hand over its primal part" % name)
     if t.shape[-1] > 1 and t.stride(-1) != 1 and t.numel():
         raise ValueError("the elements of a row of %s must lie next to each other (strides %r)" % (name, t.stride()))
     return t
@@ -68,7 +72,8 @@ def _ld(t, name):
 
 def _matrix(t, name, dtype, dev):
     """Checks a matrix argument: ``(rows, cols, leading dimension)``."""
-    if type(t) is _Tensor and (t.dtype is dtype or dtype is None and t.dtype in _DTYPES) and t.get_device() == dev and not t.requires_grad:
+    if type(t) is _Tensor and (t.dtype is dtype or dtype is None and t.dtype in _DTYPES) and t.get_device() == dev and not t.requires_grad \
+            and forward_ad._current_level < 0:
         stride = t.stride()
         if len(stride) == 2 and stride[1] == 1:
             rows, cols = t.shape

@@ -243,3 +243,23 @@ def test_entries_refuse_outputs_over_any_input():
         refused(lib.smrt_layer_norm_forward, _hip.LayerNorm(**{**norm, **kw}))
     for kw in (dict(x_scale=0xd00000, ld_x_scale=2), dict(x_scale=0xcffff0, ld_x_scale=2, dx=None), dict(x=0xd00000 - 3999 * 96 - 48, ldx=96, n=40, x_scale=0x80000, ld_x_scale=2)):
         refused(lib.smrt_layer_norm_backward, _hip.LayerNorm(**{**norm, **kw}), 0x2000000, 1 << 30)
+
+
+def test_tangents_are_refused():
+    """A dual tensor's tangent would be lost without a word.  Tensors without one are taken as ever, integers among them."""
+    from torch.autograd import forward_ad
+    cases = [(lambda d: dense(d(2, 3), t(3, 4))), (lambda d: dense(t(2, 3), d(3, 4))), (lambda d: dense(t(2, 3), t(3, 4), d(4))),
+             (lambda d: dense(t(2, 3), t(3, 4), residual=d(2, 4))), (lambda d: dense(t(2, 3), t(3, 4), out=d(2, 4))),
+             (lambda d: dense_backward(d(2, 4), t(2, 3), t(3, 4))), (lambda d: dense_backward(t(2, 4), d(2, 3), t(3, 4))),
+             (lambda d: dense_backward(t(2, 4), t(2, 3), t(3, 4), d(2, 4), activation="tanh")),
+             (lambda d: dense_grouped(t(2, 3), t(2, dtype=torch.int64), d(2, 3, 4))), (lambda d: dense_grouped(t(2, 3), t(2, dtype=torch.int64), t(2, 3, 4), d(2, 4))),
+             (lambda d: layer_norm(d(2, 3))), (lambda d: layer_norm(t(2, 3), d(3))), (lambda d: layer_norm(t(2, 3), t(3), d(3))),
+             (lambda d: layer_norm_backward(d(2, 3), t(2, 3), t(2), t(2))), (lambda d: layer_norm_backward(t(2, 3), t(2, 3), d(2), t(2))), (lambda d: pack_rows(d(2, 3)))]
+    with forward_ad.dual_level():
+        for call in cases:
+            with pytest.raises(ValueError, match="tangent"):
+                call(lambda *s: forward_ad.make_dual(t(*s), t(*s)))
+            with pytest.raises(_hip.HipLibraryError):                # past all checks of the arguments
+                call(t)
+        with pytest.raises(_hip.HipLibraryError):
+            dense_backward(t(2, 4), packed(2, 3), t(3, 4))
