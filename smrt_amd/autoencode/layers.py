@@ -21,6 +21,7 @@ import ctypes as C
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version      # a tensor of the caller's that is written over: autograd may have kept it
 
 from .. import _hip
 
@@ -257,6 +258,7 @@ def _dense(x, ends, weight, bias, residual, activation, save, out):
         if y_rows != rows or y_cols != n:
             _shape(out, "out", (rows, n))
         _on_gpu(dev)
+        increment_version(out)
         y = out
     saved, a_ptr, lda, s_ptr, lds = None, None, 0, None, 0
     if save is not None and act != 1:                      # the identity's derivative needs nothing
@@ -380,6 +382,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
         if y_rows != rows or y_cols != n:
             _shape(out, "out", (rows, n))
         _on_gpu(dev)
+        increment_version(out)
         y = out
     mean = torch.empty((rows,), dtype=torch.float32, device=device)
     rstd = torch.empty((rows,), dtype=torch.float32, device=device)

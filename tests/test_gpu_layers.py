@@ -1075,3 +1075,19 @@ def test_grouped_tiles_are_dense_tiles_for_one_group(m, k, n, dtype):
     rng = np.random.default_rng(950)
     x, w = make(rng, dtype, m, k).cuda(), make(rng, dtype, k, n).cuda()
     assert torch.equal(dense_grouped(x, torch.tensor([m], device="cuda"), w[None]), dense(x, w))
+
+
+def test_out_counts_as_written():
+    """A tensor that autograd kept and a call writes over ends its backward pass with an error, as after any in-place operation."""
+    from smrt_amd.autoencode import dense, layer_norm
+    x, w = torch.randn(6, 8, device="cuda"), torch.randn(8, 8, device="cuda")
+    for call in (lambda out: dense(x, w, out=out), lambda out: layer_norm(x, out=out), lambda out: dense(x, w, residual=out, out=out)):
+        leaf = torch.randn(6, 8, device="cuda", requires_grad=True)
+        h = torch.exp(leaf)                                  # keeps its result
+        loss = h.sum()
+        call(h.detach())
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        out = torch.empty(6, 8, device="cuda")
+        assert dense(x, w, out=out) is out
