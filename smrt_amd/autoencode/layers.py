@@ -10,8 +10,8 @@ graph (smrt/autoencode/layer.py:348-464).
     y = layer norm of x         layer_norm, layer_norm_backward
     activations in 8 bits       pack_rows, unpack_rows, PackedRows       (what the backward calls take in a tensor's place)
 
-Tensors are ``float32``, ``bfloat16`` or ``float16`` on one GPU, 2-d, with a row's elements next to each other (rows may
-be any distance apart); sums are fp32.  Work is queued on the device's current torch stream and nothing waits for it, so the calls
+Tensors are ``float32``, ``bfloat16`` or ``float16`` on one GPU, 2-d, with a row's elements next to each other and rows at
+any distance (up to 2^21 elements for what a product reads); sums are fp32.  Work is queued on the device's current torch stream and nothing waits for it, so the calls
 can be captured into graphs.  They take no part in torch's autograd -- the gradients are calls of their own -- and
 refuse a tensor that requires grad while grad mode is on, or that has a tangent.  There is no CPU fallback.
 """
@@ -79,7 +79,7 @@ def _matrix(t, name, dtype, dev):
         if len(stride) == 2 and stride[1] == 1:
             rows, cols = t.shape
             if stride[0] >= cols > 0:
-                return rows, cols, stride[0]
+                return rows, cols, stride[0] if rows > 1 else cols          # a single row has no distance to another
     _tensor(t, name, 2, dtype, dev)
     return t.shape[0], t.shape[1], _ld(t, name)
 

@@ -1091,3 +1091,18 @@ def test_out_counts_as_written():
     with torch.inference_mode():
         out = torch.empty(6, 8, device="cuda")
         assert dense(x, w, out=out) is out
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_one_row_of_a_wide_matrix(dtype):
+    """A single row has no distance to another: the width of the matrix that it is cut from does not count."""
+    from smrt_amd.autoencode import dense, dense_backward, dense_grouped
+    rng = np.random.default_rng(960)
+    x, w, g = make(rng, dtype, 1, 8), make(rng, dtype, 8, 16), make(rng, dtype, 1, 16)
+    wide = torch.zeros((2, (1 << 21) + 64), dtype=dtype, device="cuda")
+    wide[0, :8], wide[0, 8:24] = x[0].cuda(), g[0].cuda()
+    X, D = wide[:1, :8], wide[:1, 8:24]
+    y = dense(X, w.cuda())
+    check_dense(x, w, None, None, "identity", y, None, dtype)
+    check_dense_backward(g, x, w, None, "identity", *dense_backward(D, X, w.cuda()), dtype)
+    assert torch.equal(dense_grouped(X, torch.tensor([1], device="cuda"), w.cuda()[None]), y)
