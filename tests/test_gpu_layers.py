@@ -1106,3 +1106,38 @@ def test_one_row_of_a_wide_matrix(dtype):
     check_dense(x, w, None, None, "identity", y, None, dtype)
     check_dense_backward(g, x, w, None, "identity", *dense_backward(D, X, w.cuda()), dtype)
     assert torch.equal(dense_grouped(X, torch.tensor([1], device="cuda"), w.cuda()[None]), y)
+
+
+# ------------------------------------------------------------------------------------------------ fp32 products in three bf16 parts
+def worst_fp32(rng, count):
+    """fp32 numbers of one binade whose upper parts end in ones or in halves, where cutting and rounding leave the most, among ordinary ones."""
+    bits = rng.integers(0, 1 << 23, count).astype(np.uint32)
+    special = np.array([0x00ffff, 0x7fffff, 0x00ff80, 0x00ff7f, 0x007fff, 0x008000, 0x00fe80, 0x40ffff, 0x01ffff, 0x00ff81, 0x00fe7f], np.uint32)
+    some = rng.random(count) < 0.7
+    bits[some] = special[rng.integers(0, len(special), int(some.sum()))]
+    sign = rng.integers(0, 2, count).astype(np.uint32) << 31
+    return torch.from_numpy((bits | np.uint32(0x3f800000) | sign).view(np.float32))
+
+
+@pytest.mark.parametrize("m,n", [(1408, 64), (16512, 704)], ids=["64x64 tiles", "128x128 tiles"])
+def test_fp32_products_of_single_terms(m, n):
+    """Sums of one product each, from the tiles: parts are h (cut off, so m = x - h is below 2^-7 of x's power of two) and m (to nearest, so what is left is at most
+    2^-16 of it); m l + l m, which are not multiplied, come to 2^-22 = 4 u of the product.  hh and the products of the other parts are exact in fp32;
+    their sum, below 2^-6, is rounded on the way (a few u of 2^-6), and hh plus that sum once: 5.25 u altogether."""
+    from smrt_amd.autoencode import dense, dense_backward
+    rng = np.random.default_rng(910)
+    k = 16
+    one = lambda rows, cols: torch.zeros(rows, cols).scatter_(1, torch.from_numpy(rng.integers(0, cols, (rows, 1))), worst_fp32(rng, rows)[:, None])
+
+    def check(got, a, b, what):
+        want = a.double() @ b.double()                       # one term
+        close(got, want, 5.25 * U * want.abs(), what)
+    x, w, g = one(m, k), worst_fp32(rng, k * n).reshape(k, n), one(m, n)
+    check(dense(x.cuda(), w.cuda()), x, w, "y")
+    dx = dense_backward(g.cuda(), x.cuda(), w.cuda(), need_weight=False, need_bias=False)[0]
+    check(dx, g, w.T, "dx")
+    row = int(rng.integers(0, m))
+    x, g = torch.zeros(m, k), worst_fp32(rng, m * n).reshape(m, n)
+    x[row] = worst_fp32(rng, k)
+    dw = dense_backward(g.cuda(), x.cuda(), w.cuda(), need_x=False, need_bias=False)[1]
+    check(dw, x.T, g, "dw")
