@@ -283,7 +283,8 @@ int  smrt_smote_rows_f64(const double* X_dev, int64_t n_x, int64_t ldx, int64_t 
  *
  * The 8-bit form of a matrix [rows][n]: q int8 [rows][ldq], ldq >= n rounded up to 32 (the pad is zero), and one scale byte per 32
  * columns, scale [rows][ld_scale].  A value is q * 2^(byte - 127), q in [-127, 127], with the smallest power that holds the 32
- * columns' largest magnitude (not below 2^-126; 2^-24 in SMRT_F16); halves round to even.  Byte 255: the block held an infinity
+ * columns' largest magnitude (not below 2^-126; 2^-24 in SMRT_F16); halves round to even.  With the highest power, 2^122 (2^10 in SMRT_F16), q is in
+ * [-63, 63], and what would round to 64 becomes 63, since 64 of it are an infinity.  Byte 255: the block held an infinity
  * or a NaN, and all of it stands for NaN. */
 enum { SMRT_F32 = 0, SMRT_BF16 = 1, SMRT_F16 = 2 };
 

@@ -130,7 +130,9 @@ class PackedRows(object):
 
     ``q`` int8 ``[rows, cols rounded up to 32]``, ``scale`` uint8 ``[rows, cols / 32]``: 32 columns of a row share a power of two,
     a value is ``q * 2 ** (scale - 127)`` with ``|q| <= 127`` -- off by at most 1/126 of the block's largest magnitude (half a step of
-    ``q``, of which that magnitude takes 63.5 or more).  A block that held an infinity or a NaN stands for 32 NaNs (scale 255).
+    ``q``, of which that magnitude takes 63.5 or more).  The two ends of the scales differ: at the lowest (1; 103 in float16) a value is off by half of its step, 2^-127
+    (0 in float16, whose numbers are whole steps there), which takes the smallest ones to zero; at the highest (249; 137 in float16), where 64 steps would be an infinity,
+    ``|q| <= 63`` and a value is off by up to 1/64.  A block that held an infinity or a NaN stands for 32 NaNs (scale 255).
     ``dtype`` is the type of the values."""
 
     __slots__ = ("q", "scale", "cols", "dtype")

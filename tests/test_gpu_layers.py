@@ -1121,9 +1121,9 @@ def worst_fp32(rng, count):
 
 @pytest.mark.parametrize("m,n", [(1408, 64), (16512, 704)], ids=["64x64 tiles", "128x128 tiles"])
 def test_fp32_products_of_single_terms(m, n):
-    """Sums of one product each, from the tiles: parts are h (cut off, so m = x - h is below 2^-7 of x's power of two) and m (to nearest, so what is left is at most
-    2^-16 of it); m l + l m, which are not multiplied, come to 2^-22 = 4 u of the product.  hh and the products of the other parts are exact in fp32;
-    their sum, below 2^-6, is rounded on the way (a few u of 2^-6), and hh plus that sum once: 5.25 u altogether."""
+    """Sums of one product each, from the tiles: parts are h (cut off, so m = x - h is at most 2^-7 of x's power of two) and m (cut off in one operand, away from zero in
+    the other), which leaves l below 2^-15.  m l and l m, which are not multiplied, have different signs and stay below 2^-22 = 4 u of the product.  hh and the
+    products of the other parts are exact in fp32; their sum, below 2^-6, is rounded on the way (a few u of 2^-6), and hh plus that sum once: 5.25 u altogether."""
     from smrt_amd.autoencode import dense, dense_backward
     rng = np.random.default_rng(910)
     k = 16
@@ -1141,3 +1141,29 @@ def test_fp32_products_of_single_terms(m, n):
     x[row] = worst_fp32(rng, k)
     dw = dense_backward(g.cuda(), x.cuda(), w.cuda(), need_x=False, need_bias=False)[1]
     check(dw, x.T, g, "dw")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_pack_holds_its_bounds(dtype):
+    """1/126 of a block's largest magnitude at every scale but the ends: half a step at the lowest (every f16 number there is a whole number of steps), 1/64 at the
+    highest, whose 64 steps would be an infinity."""
+    from smrt_amd.autoencode import pack_rows, unpack_rows
+    rng = np.random.default_rng(970)
+    low, high = (-24, 10) if dtype == F16 else (-126, 122)
+    top = torch.finfo(dtype).max
+    exps = rng.integers(-24 if dtype == F16 else -149, 16 if dtype == F16 else 128, 4000)
+    x = torch.from_numpy((rng.uniform(-1, 1, (4000, 32)) * np.exp2(exps)[:, None]).clip(-top, top)).to(dtype)
+    step = 2.0 ** high
+    ends = [[top], [-top, top / 2, step, 0.5 * step], [63.5 * step], [63.49 * step], [127.0 * step / 2], [127.02 * step / 2], [2.0 ** low], [2.0 ** low / 2],
+            [2.0 ** low / 2, 2.0 ** low * 1.5], [2.0 ** low / 4], [127 * 2.0 ** low, 2.0 ** low / 2], [63.5 * 2.0 ** low]]
+    for i, e in enumerate(ends):
+        x[i] = 0
+        x[i, :len(e)] = torch.tensor(e, dtype=torch.float64).clamp(-top, top).to(dtype)
+    p = pack_rows(x.cuda())
+    v, X, byte = unpack_rows(p).cpu().double(), x.double(), p.scale.cpu().int()
+    assert v.isfinite().all() and (p.q.cpu().int().abs()[byte[:, 0] == high + 127] <= 63).all()
+    most = X.abs().amax(1, keepdim=True)
+    bound = torch.where(byte == high + 127, most / 64, torch.where(byte == low + 127, 0.0 if dtype == F16 else 2.0 ** (low - 1), most / 126))
+    assert ((v - X).abs() <= bound).all()
+    for b in (low + 127, low + 128, 127, high + 126, high + 127):
+        assert (byte == b).any(), b
