@@ -321,7 +321,10 @@ def dense_backward(grad, x, weight, saved=None, activation="identity", need_x=Tr
     """Gradients ``(dx, dweight, dbias)`` of ``dense`` from ``grad`` = d loss / d y (None where not needed; the residual's gradient is ``grad``).
 
     ``x`` and ``saved`` are the forward pass's tensors, or their 8-bit forms: the gradients are then those at the values the 8 bits
-    stand for."""
+    stand for.
+
+    In a 16-bit type ``dz = grad * act'`` is rounded once to that type before it is multiplied into ``dx`` and ``dweight``, as an operand of the matrix cores; ``dbias`` is
+    summed from the values before.  Kernels for a few rows (at most 256) multiply ``dz`` in fp32."""
     return _dense_backward(grad, x, None, weight, saved, activation, need_x, need_weight, need_bias)
 
 
@@ -335,7 +338,7 @@ def dense_grouped(x, ends, weight, bias=None, residual=None, activation="identit
 
 def dense_grouped_backward(grad, x, ends, weight, saved=None, activation="identity", need_x=True, need_weight=True, need_bias=True):
     """Gradients ``(dx [rows, k], dweight [groups, k, n], dbias [groups, n])`` of ``dense_grouped``; zero for a class without rows, and
-    for rows that are in no class."""
+    for rows that are in no class.  ``dz`` is rounded as in ``dense_backward``."""
     return _dense_backward(grad, x, _ends(ends), weight, saved, activation, need_x, need_weight, need_bias)
 
 

@@ -17,7 +17,9 @@ constexpr int MAX_GROUPS = 65535;
 
 // ------------------------------------------------------------------------------------------------ dz = g * act'(a), column sums
 // One pass over g (and a): writes dz for the two products that read it, and sums its columns into db on the way (in fp32, from
-// the values before they are rounded to T).  A workgroup has 256 columns of a chunk of DZ_CHUNK rows (chunk_rows), 8 rows x 4 at a time.
+// the values before they are rounded to T).  dz itself is rounded to T, because the matrix cores take 16-bit operands: two parts of it would
+// double both products and the bytes between the launches.  From the result in 64 bits, dx and dW of 32768 x 1024 x 1024 bf16 elu are off by 1.86e-3 of their norm, where rounding them alone
+// is 1.66e-3 (sigmoid 2.3e-3; relu and the identity, whose dz is g or 0, 1.66e-3).  The kernels for a few rows multiply dz in fp32 (layer_rows.hpp).  A workgroup has 256 columns of a chunk of DZ_CHUNK rows (chunk_rows), 8 rows x 4 at a time.
 // (with chunks of 256 rows, which need no join at 256 x 784 x 450, the step's three launches there took 35 us instead of 21)
 constexpr int DZ_CHUNK = 64;
 struct DzArgs {
