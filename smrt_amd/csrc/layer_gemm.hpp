@@ -13,7 +13,8 @@
 // 0 on average, 0.37 u in the root mean square over random numbers, where rounding an fp32 product is 0.42 u.  (With m cut off in both they reach 7.8 u, always of the product's
 // sign, 0.63 u on average; a step of 40000 x 784 x 450 in 8 groups 921 us, this 933, both rounded to nearest 946.)
 // hh is summed apart from the small terms: the small ones keep their bits, and where
-// hh alone is an infinity or NaN (whose parts m, l are NaN) it is the answer.
+// hh alone is an infinity or NaN (whose parts m, l are NaN) it is the answer.  (h of a NaN that has no bit of its payload in the upper half, which no operation
+// yields, is an infinity.)
 #pragma once
 #include "layer_join.hpp"
 
